@@ -388,6 +388,141 @@ int pvlc_linear(const pvlc_half* x, uint32_t rows, uint32_t ldx, const pvlc_half
                 uint32_t k, uint32_t gate, uint32_t split, pvlc_half* out, uint32_t ldo,
                 void* stream);
 
+/* ----------------------------------------------------------------------------
+ * 8-bit paged KV cache, and the selection step of a beam search over it.
+ * They have no counterpart in the reference, whose caches are contiguous fp16
+ * or f32 and whose search is greedy.
+ *
+ * A page holds PVLC_KV8_PAGE = 32 consecutive rows of one sequence, every KV
+ * head, K and V, in 8-bit codes of type code_type.  One (page, K or V, head)
+ * block X of 32 x 128 values has one scale 2^e, e the smallest integer with
+ * max|X| <= Q 2^e (Q = 448 for e4m3, 127 for int8; scale 1 for a block of
+ * zeros), and code = X / 2^e rounded to nearest, ties to even.  A block with a
+ * NaN or an infinity has scale NaN and codes 0.  The tokens % 32 rows of a
+ * sequence's open block stay fp16 in its slot's tail until it is full; every
+ * value is rounded to 8 bits once, however its rows arrived.
+ *
+ * A slot is a sequence's row of `table`, `tokens` and `tails`: table[s][j] is
+ * the page of its rows 32 j .. 32 j + 31, for j < tokens[s] / 32, and beyond
+ * those a page that the next blocks will fill, or -1.  refs[p] counts the
+ * slots that name page p; 0 is a free page.  A cache starts with table -1,
+ * tokens and refs 0.  A slot with 0 tokens that no call names is free.
+ * head_dim is 128.  Every call takes sequences as `slot[batch]`: distinct slots,
+ * or -1 for an idle sequence, which is passed over (its outputs are left as
+ * they were).  All arrays are device memory; the struct itself is read during
+ * the call only.
+ */
+#define PVLC_KV8_PAGE 32u
+#define PVLC_KV8_E4M3 0u
+#define PVLC_KV8_INT8 1u
+#define PVLC_KV8_MAX_BATCH 2048u
+#define PVLC_KV8_MAX_KV_HEADS 16u
+#define PVLC_KV8_MAX_GROUP 16u          /* query heads of one KV head */
+#define PVLC_KV8_MAX_SLOTS 65536u
+#define PVLC_KV8_MAX_PAGES_PER_SLOT 1048576u
+#define PVLC_KV8_MAX_LAYERS 1024u
+typedef struct pvlc_kv8_cache {
+  void* codes;       /* [layers][pages][2][kv_heads][32][128], 16-byte aligned */
+  float* scales;     /* [layers][pages][kv_heads][2] (K, V), 8-byte aligned */
+  pvlc_half* tails;  /* [layers][slots][2][kv_heads][32][128], 16-byte aligned */
+  int32_t* table;    /* [slots][max_pages] */
+  int32_t* tokens;   /* [slots] */
+  int32_t* refs;     /* [pages] */
+  uint32_t layers, pages, slots, max_pages, kv_heads, code_type;
+} pvlc_kv8_cache;
+
+/* Scratch of the kv8 calls on caches of up to `pages` pages and `slots` slots,
+ * for batches of up to `batch` sequences and `query_heads` heads (0 when they
+ * are out of range).  Zeroed once with pvlc_attn_kv8_workspace_init; reusable
+ * on one stream, not by calls that may overlap.  pvlc_attn_kv8_errors waits
+ * for the stream, reads and clears the fault word: bit 0 a slot's row count or
+ * capacity, bit 1 a rope row, bit 3 a pipeline wait that timed out, bit 4 a
+ * page id, bit 5 a slot or parent, bit 6 no free page or slot, bit 7 the
+ * input's row range. */
+size_t pvlc_attn_kv8_workspace_bytes(uint32_t batch, uint32_t query_heads, uint32_t kv_heads,
+                                     uint32_t slots, uint32_t pages);
+int pvlc_attn_kv8_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
+int pvlc_attn_kv8_errors(void* workspace, uint32_t* flags_out, void* stream);
+
+/* Appends rows to sequences, in one layer: sequence b takes the count[b] <=
+ * max_count rows k, v + (begin[b] + i) * row_stride ([kv_heads, 128] each,
+ * keys rotated) behind its tokens[slot[b]] rows.  Full blocks go into the
+ * pages that the table names (pvlc_attn_kv8_grow gives them), the rest into
+ * the tail.  `rows` is the number of rows in k and v.  tokens is not advanced:
+ * it serves every layer.  A sequence with a bad slot, row range or count is
+ * flagged and left out; a block whose page is bad is flagged and not stored. */
+int pvlc_attn_kv8_store(const pvlc_kv8_cache* cache, uint32_t layer, const pvlc_half* k,
+                        const pvlc_half* v, uint32_t rows, uint32_t row_stride,
+                        const int32_t* begin, const int32_t* count, const int32_t* slot,
+                        uint32_t batch, uint32_t max_count, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* One token of every sequence in one layer, as pvlc_attn_decode_strided:
+ * q [batch, query_heads, 128] and k_new, v_new [batch, kv_heads, 128] before
+ * RoPE (rows q_row_stride / kv_row_stride elements apart, multiples of 8),
+ * rotated with table row rope_row[b] (tokens[slot[b]] when rope_row is NULL).
+ * The rotated key and the value become row tokens % 32 of the tail, attention
+ * runs over the tokens / 32 pages and the tail up to that row, and a tail that
+ * this row fills is quantised into its page.  query_heads = kv_heads x group,
+ * group <= 16.  slot NULL: sequence b is slot b.  tokens is not advanced.  A
+ * sequence with a bad slot, row count or rope row is flagged and its output
+ * zero; a bad page id is flagged and its rows read as NaN. */
+int pvlc_attn_kv8_decode(const pvlc_kv8_cache* cache, uint32_t layer, const pvlc_half* q,
+                         uint32_t q_row_stride, const pvlc_half* k_new, const pvlc_half* v_new,
+                         uint32_t kv_row_stride, uint32_t query_heads, const float* rope_cos,
+                         const float* rope_sin, uint32_t rope_rows, const int32_t* rope_row,
+                         const int32_t* slot, uint32_t batch, void* workspace,
+                         size_t workspace_bytes, pvlc_half* out, void* stream);
+
+/* tokens[slot[b]] += advance[b], then gives every sequence the pages that it
+ * lacks for its next ahead[b] rows (full blocks only), lowest free id first,
+ * in sequence order.  advance / ahead NULL: advance_by / ahead_by for all.
+ * When a slot is bad or named twice, or rows exceed 32 max_pages + 31, the call
+ * is flagged and changes nothing; when pages run out, the last sequences'
+ * table entries stay -1. */
+int pvlc_attn_kv8_grow(const pvlc_kv8_cache* cache, const int32_t* slot, uint32_t batch,
+                       const int32_t* advance, uint32_t advance_by, const int32_t* ahead,
+                       uint32_t ahead_by, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Reorders, duplicates and drops sequences (a beam search's step): sequence b
+ * becomes a copy of sequence parent[b] (an index into slot; -1: none).  First
+ * every sequence's tokens grow by advance_by.  The lowest b with a parent keeps
+ * the parent's slot; each other child takes the lowest free slot, in order,
+ * sharing the parent's full pages and copying its open block in every layer.
+ * A sequence that is no parent gives its slot and pages back.  slot_out[b] is
+ * the new slot, -1 for none or when slots ran out (flagged); it may not overlap
+ * slot or parent.  A bad or repeated slot or a bad parent is flagged and the
+ * call changes nothing (slot_out = slot). */
+int pvlc_attn_kv8_fork(const pvlc_kv8_cache* cache, const int32_t* slot, const int32_t* parent,
+                       uint32_t batch, uint32_t advance_by, int32_t* slot_out, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Copies a cache's live pages (refs > 0), in order, to pages 0, 1, .. of
+ * another cache with the same layers, heads and type and at least as many
+ * slots; its tables, counts, references and tails are made to match.  *live_out
+ * (device, may be NULL) is the number of live pages.  If they, or a slot's
+ * rows, do not fit, the call is flagged, changes nothing and *live_out is -1. */
+int pvlc_attn_kv8_compact(const pvlc_kv8_cache* from, const pvlc_kv8_cache* into,
+                          int32_t* live_out, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* The best topk continuations of every request: out_*[batch, topk], best first,
+ * of the beams x vocab candidates scores[r][w] + x[v] - log sum exp(x), x the
+ * logits row r * beams + w (f32, or fp16 with half_logits = 1; rows row_stride
+ * elements apart).  Scores are computed and compared in f64; equal ones go to
+ * the lower beam, then the larger logit, then the lower token.  A NaN logit or
+ * candidate counts as -infinity.  The workspace needs no initialisation. */
+#define PVLC_BEAM_MAX_BEAMS 32u
+#define PVLC_BEAM_MAX_TOPK 64u
+#define PVLC_BEAM_MAX_VOCAB 16777216u
+size_t pvlc_lm_head_beam_topk_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab,
+                                              uint32_t topk);
+int pvlc_lm_head_beam_topk(const void* logits, uint32_t half_logits, uint64_t row_stride,
+                           const float* scores, uint32_t batch, uint32_t beams, uint32_t vocab,
+                           uint32_t topk, void* workspace, size_t workspace_bytes,
+                           float* out_score, int32_t* out_beam, int32_t* out_token,
+                           void* stream);
+
 /* ---- model packs: BLAKE3 section digests on the device ----------------- */
 /* BLAKE3 (plain hash mode, 32-byte output) of `bytes` bytes of device memory
  * at `data`: the checksum every .pvlc pack directory entry carries for its

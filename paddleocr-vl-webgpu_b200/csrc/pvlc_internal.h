@@ -126,6 +126,60 @@ bool linear_split_fits(uint32_t rows, uint32_t k, uint32_t split);
 int linear_launch(const LinearArgs& a, cudaStream_t stream);
 int linear_fault_word(uint32_t* out, cudaStream_t s);
 
+// 8-bit paged KV cache (kv8_store.cu, kv8_decode.cu, kv8_pages.cu).
+struct Kv8StoreArgs {
+  const pvlc_half* k;
+  const pvlc_half* v;
+  uint32_t rows, row_stride;
+  const int32_t* begin;
+  const int32_t* count;
+  const int32_t* slot;
+  uint32_t batch, max_count;
+  void* workspace;
+};
+struct Kv8DecodeArgs {
+  const pvlc_half* q;
+  const pvlc_half* k_new;
+  const pvlc_half* v_new;
+  const float* rope_cos;
+  const float* rope_sin;
+  const int32_t* rope_row;
+  const int32_t* slot;
+  pvlc_half* out;
+  uint32_t q_stride, kv_stride, rope_rows, batch, query_heads;
+  void* workspace;
+};
+int32_t* kv8_scratch(void* workspace);     // behind the tickets
+uint32_t* kv8_tickets(void* workspace);    // zero between calls
+size_t kv8_decode_scratch_bytes(uint32_t batch, uint32_t query_heads, uint32_t kv_heads);
+int kv8_store_launch(const pvlc_kv8_cache& c, uint32_t layer, const Kv8StoreArgs& a,
+                     cudaStream_t stream);
+int kv8_decode_launch(const pvlc_kv8_cache& c, uint32_t layer, const Kv8DecodeArgs& a,
+                      cudaStream_t stream);
+int kv8_grow_launch(const pvlc_kv8_cache& c, const int32_t* slot, uint32_t batch,
+                    const int32_t* advance, int32_t advance_by, const int32_t* ahead,
+                    int32_t ahead_by, void* workspace, cudaStream_t stream);
+int kv8_fork_launch(const pvlc_kv8_cache& c, const int32_t* slot, const int32_t* parent,
+                    uint32_t batch, int32_t advance_by, int32_t* slot_out, void* workspace,
+                    cudaStream_t stream);
+int kv8_compact_launch(const pvlc_kv8_cache& from, const pvlc_kv8_cache& into, int32_t* live_out,
+                       void* workspace, cudaStream_t stream);
+
+// Beam selection over logits (beam_topk.cu).
+struct BeamArgs {
+  const void* logits;
+  uint32_t half_logits;
+  uint64_t ld;
+  const float* scores;
+  uint32_t batch, beams, vocab, topk;
+  void* workspace;
+  float* out_score;
+  int32_t* out_beam;
+  int32_t* out_token;
+};
+size_t beam_topk_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t topk);
+int beam_topk_launch(const BeamArgs& a, cudaStream_t stream);
+
 int device_sm_count();
 // The current device's SM count, or the B200's 148 when no GPU is visible.
 int sms_or_default_count();

@@ -59,6 +59,14 @@ class Plan(ctypes.Structure):
     ]
 
 
+class Kv8CacheStruct(ctypes.Structure):
+    """pvlc_kv8_cache: the device arrays and sizes of an 8-bit paged KV cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("codes", "scales", "tails", "table", "tokens", "refs")] + \
+               [(n, ctypes.c_uint32) for n in
+                ("layers", "pages", "slots", "max_pages", "kv_heads", "code_type")]
+
+
 _P = ctypes.c_void_p
 _U32 = ctypes.c_uint32
 _SIGNATURES = {
@@ -101,6 +109,20 @@ _SIGNATURES = {
                                          _P]),
     "pvlc_lm_head_top1_errors": (ctypes.c_int, [_P, _U32, ctypes.POINTER(ctypes.c_uint32), _P]),
     "pvlc_linear": (ctypes.c_int, [_P, _U32, _U32, _P, _U32, _U32, _U32, _U32, _P, _U32, _P]),
+    "pvlc_attn_kv8_workspace_bytes": (ctypes.c_size_t, [_U32] * 5),
+    "pvlc_attn_kv8_workspace_init": (ctypes.c_int, [_P, ctypes.c_size_t, _P]),
+    "pvlc_attn_kv8_errors": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_uint32), _P]),
+    "pvlc_attn_kv8_store": (ctypes.c_int, [_P, _U32, _P, _P, _U32, _U32, _P, _P, _P, _U32, _U32,
+                                           _P, ctypes.c_size_t, _P]),
+    "pvlc_attn_kv8_decode": (ctypes.c_int, [_P, _U32, _P, _U32, _P, _P, _U32, _U32, _P, _P, _U32,
+                                            _P, _P, _U32, _P, ctypes.c_size_t, _P, _P]),
+    "pvlc_attn_kv8_grow": (ctypes.c_int, [_P, _P, _U32, _P, _U32, _P, _U32, _P, ctypes.c_size_t,
+                                          _P]),
+    "pvlc_attn_kv8_fork": (ctypes.c_int, [_P, _P, _P, _U32, _U32, _P, _P, ctypes.c_size_t, _P]),
+    "pvlc_attn_kv8_compact": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "pvlc_lm_head_beam_topk_workspace_bytes": (ctypes.c_size_t, [_U32] * 4),
+    "pvlc_lm_head_beam_topk": (ctypes.c_int, [_P, _U32, ctypes.c_uint64, _P, _U32, _U32, _U32,
+                                              _U32, _P, ctypes.c_size_t, _P, _P, _P, _P]),
     "pvlc_plan_vision_varlen": (ctypes.c_int, [_P, _U32, _U32, _U32, _U32, ctypes.POINTER(Plan)]),
     "pvlc_plan_decoder_prefill": (ctypes.c_int, [_U32, _U32, _U32, ctypes.POINTER(Plan)]),
     "pvlc_plan_decoder_kv_session": (ctypes.c_int, [_U32, _U32, _U32, _U32, _U32,

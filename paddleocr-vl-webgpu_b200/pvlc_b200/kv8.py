@@ -1,0 +1,284 @@
+"""8-bit paged KV cache: store, single-token decode, grow, fork and compact.
+
+A `Cache` holds the pages of every decoder layer in 8-bit codes (e4m3 or int8) with one
+power-of-two scale per (page, K or V, KV head), the fp16 rows of each sequence's open block,
+and the device-side page tables.  The C ABI (include/pvlc_cuda_attn.h) defines the layout and
+the arithmetic; every function here checks placement, type and shape, then enqueues one call
+on the current CUDA stream.  Sequences are named by slot tensors (int32, distinct, -1: idle).
+
+A prompt goes in with grow(ahead=rows), store() per layer, grow(advance=rows, ahead=1); a
+decode step is decode() per layer, then grow(advance=1, ahead=1) -- or, in a beam search,
+ops.beam_topk, fork(advance=1), grow(ahead=1).  None of it waits for the host, so a step can
+be captured in a CUDA graph.  Faults that only the device can see (a slot out of range, pages
+exhausted) skip the work and set a bit of Workspace.errors().
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import abi
+
+PAGE, HD = 32, 128                       # rows of a page, head dimension
+CODE_TYPES = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+# Workspace.errors() bits
+FLAG_ROWS_HELD, FLAG_ROPE_ROW, FLAG_TIMEOUT = 1, 2, 8
+FLAG_PAGE, FLAG_SLOT, FLAG_EXHAUSTED, FLAG_INPUT_ROWS = 16, 32, 64, 128
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _need(t, dtype, shape, device, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _rows(t, heads, device, name):
+    """A [rows, heads, 128] fp16 tensor whose rows may sit apart; the stride in elements."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype is not torch.float16:
+        raise TypeError(f"{name} must be torch.float16, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != HD:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected (rows, {heads}, {HD})")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (heads > 1 and s1 != HD):
+        raise ValueError(f"{name}: each row must be contiguous")
+    if t.shape[0] == 1:
+        return heads * HD
+    if s0 >= 1 << 32:
+        raise ValueError(f"{name}: rows are too far apart")
+    return s0
+
+
+class Cache:
+    """The device arrays of an 8-bit paged KV cache (the C ABI's pvlc_kv8_cache).
+
+    codes [layers, pages, 2, kv_heads, 32, 128] (torch.float8_e4m3fn or torch.int8), scales
+    [layers, pages, kv_heads, 2] f32, tails [layers, slots, 2, kv_heads, 32, 128] fp16, table
+    [slots, max_pages], tokens [slots] and refs [pages] int32; all contiguous, on one device.
+    Cache.empty() makes one with no sequences."""
+
+    def __init__(self, codes, scales, tails, table, tokens, refs):
+        if not isinstance(codes, torch.Tensor) or not codes.is_cuda:
+            raise TypeError("codes must be a CUDA tensor")
+        if codes.dtype not in CODE_TYPES:
+            raise TypeError(f"codes must be float8_e4m3fn or int8, got {codes.dtype}")
+        if codes.dim() != 6 or codes.shape[2] != 2 or codes.shape[4:] != (PAGE, HD):
+            raise ValueError("codes must be [layers, pages, 2, kv_heads, 32, 128], got "
+                             f"{tuple(codes.shape)}")
+        if not isinstance(table, torch.Tensor) or table.dim() != 2:
+            raise ValueError("table must be [slots, max_pages]")
+        L, P, _, H = codes.shape[:4]
+        S, M = table.shape
+        self.device = dev = codes.device
+        _need(codes, codes.dtype, codes.shape, dev, "codes")
+        _need(scales, torch.float32, (L, P, H, 2), dev, "scales")
+        _need(tails, torch.float16, (L, S, 2, H, PAGE, HD), dev, "tails")
+        _need(table, torch.int32, (S, M), dev, "table")
+        _need(tokens, torch.int32, (S,), dev, "tokens")
+        _need(refs, torch.int32, (P,), dev, "refs")
+        self.codes, self.scales, self.tails = codes, scales, tails
+        self.table, self.tokens, self.refs = table, tokens, refs
+        self.layers, self.pages, self.slots, self.max_pages, self.kv_heads = L, P, S, M, H
+        self._c = abi.Kv8CacheStruct(*[t.data_ptr() for t in (codes, scales, tails, table,
+                                                              tokens, refs)],
+                                     L, P, S, M, H, CODE_TYPES[codes.dtype])
+        self._p = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, layers: int, pages: int, slots: int, max_pages: int, kv_heads: int = 2,
+              dtype=torch.float8_e4m3fn, device=None) -> "Cache":
+        dev = torch.device(device or "cuda")
+        ints = dict(dtype=torch.int32, device=dev)
+        return cls(torch.empty((layers, pages, 2, kv_heads, PAGE, HD), dtype=dtype, device=dev),
+                   torch.empty((layers, pages, kv_heads, 2), dtype=torch.float32, device=dev),
+                   torch.empty((layers, slots, 2, kv_heads, PAGE, HD), dtype=torch.float16,
+                               device=dev),
+                   torch.full((slots, max_pages), -1, **ints), torch.zeros(slots, **ints),
+                   torch.zeros(pages, **ints))
+
+    def reset(self):
+        """Drop every sequence: all pages and slots are free again."""
+        self.table.fill_(-1)
+        self.tokens.zero_()
+        self.refs.zero_()
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in
+                   (self.codes, self.scales, self.tails, self.table, self.tokens, self.refs))
+
+
+class Workspace:
+    """Device scratch and fault word of the calls on caches up to this one's sizes, for
+    batches up to `batch` sequences of `query_heads` heads.  One stream at a time."""
+
+    def __init__(self, cache: Cache, batch: int, query_heads: int | None = None):
+        self.device = cache.device
+        self.nbytes = int(abi.lib().pvlc_attn_kv8_workspace_bytes(
+            int(batch), int(query_heads or cache.kv_heads), cache.kv_heads, cache.slots,
+            cache.pages))
+        if not self.nbytes:
+            raise abi.PvlcError(abi.INVALID_DECODER_GEOMETRY, "pvlc_attn_kv8_workspace_bytes")
+        self.buffer = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device)
+        self._p = self.buffer.data_ptr()
+        with torch.cuda.device(self.device):
+            abi.check(abi.lib().pvlc_attn_kv8_workspace_init(self._p, self.nbytes, _stream()),
+                      "pvlc_attn_kv8_workspace_init")
+
+    def errors(self) -> int:
+        """Read and clear the fault word (FLAG_* bits); waits for the current stream."""
+        flags = ctypes.c_uint32(0)
+        st = abi.lib().pvlc_attn_kv8_errors(self._p, ctypes.byref(flags), _stream())
+        if st not in (abi.OK, abi.DEVICE_FAULT_FLAG):
+            abi.check(st, "pvlc_attn_kv8_errors")
+        return int(flags.value)
+
+
+def _call(cache, workspace, *others):
+    """The checks that every call shares: one device, and that the current one."""
+    if not isinstance(cache, Cache) or not isinstance(workspace, Workspace):
+        raise TypeError("expected a kv8.Cache and a kv8.Workspace")
+    if workspace.device != cache.device:
+        raise ValueError(f"the workspace is on {workspace.device}, the cache on {cache.device}")
+    if cache.device.index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on {cache.device}, which is not the current device")
+
+
+def store(cache: Cache, layer: int, k, v, begin, count, slot, max_count: int,
+          workspace: Workspace):
+    """Append rows to sequences in one layer (pvlc_attn_kv8_store).
+
+    k, v: [rows, kv_heads, 128] fp16, keys rotated, rows the same distance apart in both;
+    sequence b takes rows begin[b] : begin[b] + count[b] (int32 device tensors, count <=
+    max_count) behind the rows its slot holds."""
+    _call(cache, workspace)
+    dev = cache.device
+    ks, vs = _rows(k, cache.kv_heads, dev, "k"), _rows(v, cache.kv_heads, dev, "v")
+    if ks != vs or k.shape[0] != v.shape[0]:
+        raise ValueError("k and v must have the same rows, the same distance apart")
+    B = slot.shape[0]
+    _need(slot, torch.int32, (B,), dev, "slot")
+    _need(begin, torch.int32, (B,), dev, "begin")
+    _need(count, torch.int32, (B,), dev, "count")
+    if not 0 <= layer < cache.layers or max_count < 0:
+        raise ValueError("layer or max_count out of range")
+    st = abi.lib().pvlc_attn_kv8_store(
+        cache._p, layer, k.data_ptr(), v.data_ptr(), k.shape[0], ks, begin.data_ptr(),
+        count.data_ptr(), slot.data_ptr(), B, max_count, workspace._p, workspace.nbytes,
+        _stream())
+    abi.check(st, "pvlc_attn_kv8_store")
+
+
+def decode(cache: Cache, layer: int, q, k_new, v_new, rope_cos, rope_sin, slot,
+           workspace: Workspace, rope_row=None, out=None):
+    """One token of every sequence in one layer, M-RoPE and append fused
+    (pvlc_attn_kv8_decode).
+
+    q [B, query_heads, 128], k_new, v_new [B, kv_heads, 128] fp16 before RoPE, each possibly a
+    row-strided view (column blocks of one projection; k_new and v_new alike); rope tables
+    [3, R, 128] f32; rope_row int32 [B] (None: the rows the slot holds); slot int32 [B] (None:
+    sequence b is slot b).  Returns [B, query_heads, 128] fp16."""
+    _call(cache, workspace)
+    dev, H = cache.device, cache.kv_heads
+    B, QH = q.shape[0], q.shape[1]
+    qs = _rows(q, QH, dev, "q")
+    ks, vs = _rows(k_new, H, dev, "k_new"), _rows(v_new, H, dev, "v_new")
+    if ks != vs or k_new.shape[0] != B or v_new.shape[0] != B:
+        raise ValueError("k_new and v_new must have q's rows, the same distance apart")
+    R = rope_cos.shape[1]
+    _need(rope_cos, torch.float32, (3, R, HD), dev, "rope_cos")
+    _need(rope_sin, torch.float32, (3, R, HD), dev, "rope_sin")
+    sp = rp = None
+    if slot is not None:
+        _need(slot, torch.int32, (B,), dev, "slot")
+        sp = slot.data_ptr()
+    if rope_row is not None:
+        _need(rope_row, torch.int32, (B,), dev, "rope_row")
+        rp = rope_row.data_ptr()
+    if out is None:
+        out = torch.empty((B, QH, HD), dtype=torch.float16, device=dev)
+    else:
+        _need(out, torch.float16, (B, QH, HD), dev, "out")
+    if not 0 <= layer < cache.layers:
+        raise ValueError("layer out of range")
+    st = abi.lib().pvlc_attn_kv8_decode(
+        cache._p, layer, q.data_ptr(), qs, k_new.data_ptr(), v_new.data_ptr(), ks, QH,
+        rope_cos.data_ptr(), rope_sin.data_ptr(), R, rp, sp, B, workspace._p, workspace.nbytes,
+        out.data_ptr(), _stream())
+    abi.check(st, "pvlc_attn_kv8_decode")
+    return out
+
+
+def _amount(x, B, dev, name):
+    """(device pointer, 0) of a per-sequence tensor, or (None, rows) of one number."""
+    if isinstance(x, torch.Tensor):
+        _need(x, torch.int32, (B,), dev, name)
+        return x.data_ptr(), 0
+    if not 0 <= x < 1 << 31:
+        raise ValueError(f"{name} out of range")
+    return None, x
+
+
+def grow(cache: Cache, slot, workspace: Workspace, advance=0, ahead=0):
+    """Advance sequences by `advance` rows and give them the pages of their next `ahead` rows
+    (each a number, or an int32 tensor per sequence; pvlc_attn_kv8_grow)."""
+    _call(cache, workspace)
+    B = slot.shape[0]
+    _need(slot, torch.int32, (B,), cache.device, "slot")
+    ap, an = _amount(advance, B, cache.device, "advance")
+    hp, hn = _amount(ahead, B, cache.device, "ahead")
+    st = abi.lib().pvlc_attn_kv8_grow(cache._p, slot.data_ptr(), B, ap, an, hp, hn, workspace._p,
+                                      workspace.nbytes, _stream())
+    abi.check(st, "pvlc_attn_kv8_grow")
+
+
+def fork(cache: Cache, slot, parent, workspace: Workspace, advance: int = 0, out=None):
+    """Sequence b becomes a copy of sequence parent[b] (int32 [B], -1: none), after every
+    sequence has grown by `advance` rows; returns the new slots (pvlc_attn_kv8_fork)."""
+    _call(cache, workspace)
+    dev, B = cache.device, slot.shape[0]
+    _need(slot, torch.int32, (B,), dev, "slot")
+    _need(parent, torch.int32, (B,), dev, "parent")
+    if out is None:
+        out = torch.empty_like(slot)
+    else:
+        _need(out, torch.int32, (B,), dev, "out")
+    if not 0 <= advance < 1 << 31:
+        raise ValueError("advance out of range")
+    st = abi.lib().pvlc_attn_kv8_fork(cache._p, slot.data_ptr(), parent.data_ptr(), B, advance,
+                                      out.data_ptr(), workspace._p, workspace.nbytes, _stream())
+    abi.check(st, "pvlc_attn_kv8_fork")
+    return out
+
+
+def compact(cache: Cache, into: Cache, workspace: Workspace, live=None):
+    """Copy the live pages, in order, to the front of another cache with the same layers,
+    heads and type, and make its tables match (pvlc_attn_kv8_compact).  live: optional int32
+    [1] tensor that receives the number of live pages (-1: they do not fit)."""
+    _call(cache, workspace)
+    if not isinstance(into, Cache):
+        raise TypeError("into must be a kv8.Cache")
+    if into.device != cache.device:
+        raise ValueError(f"into is on {into.device}, the cache on {cache.device}")
+    if live is not None:
+        _need(live, torch.int32, (1,), cache.device, "live")
+    st = abi.lib().pvlc_attn_kv8_compact(cache._p, into._p,
+                                         live.data_ptr() if live is not None else None,
+                                         workspace._p, workspace.nbytes, _stream())
+    abi.check(st, "pvlc_attn_kv8_compact")

@@ -415,3 +415,57 @@ def lm_head_top1(hidden, lm_head, tokens=None, logits=None, workspace=None):
             _ptr(logits[r0:r1] if logits is not None else None), _stream())
         abi.check(st, "pvlc_lm_head_top1")
     return tokens
+
+
+class BeamWorkspace:
+    """Device scratch of beam_topk for calls up to these sizes."""
+
+    def __init__(self, batch: int, beams: int, vocab: int, topk: int, device=None):
+        self.nbytes = int(abi.lib().pvlc_lm_head_beam_topk_workspace_bytes(batch, beams, vocab,
+                                                                           topk))
+        if not self.nbytes:
+            raise abi.PvlcError(abi.INVALID_DECODER_GEOMETRY,
+                                "pvlc_lm_head_beam_topk_workspace_bytes")
+        self.buffer = torch.empty(self.nbytes, dtype=torch.uint8,
+                                  device=device or torch.device("cuda"))
+
+
+def beam_topk(logits, scores, topk: int, workspace: BeamWorkspace | None = None, out=None):
+    """The best `topk` continuations of every request's beams (pvlc_lm_head_beam_topk):
+    logits [B * W, vocab] f32 or fp16 (rows may be pitched), scores [B, W] f32 -> (score
+    [B, topk] f32, beam [B, topk] int32, token [B, topk] int32), best first, of the candidates
+    scores[r, w] + log_softmax(logits[r W + w]).  Equal scores go to the lower beam, then the
+    larger logit, then the lower token; NaN counts as -infinity.  out: the three tensors."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise TypeError("logits must be a CUDA tensor")
+    if logits.dtype not in (torch.float32, torch.float16):
+        raise TypeError(f"logits must be float32 or float16, got {logits.dtype}")
+    dev = logits.device
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"logits are on {dev}, which is not the current device")
+    if scores.dim() != 2 or logits.dim() != 2:
+        raise ValueError("logits must be [B * W, vocab] and scores [B, W]")
+    B, W = scores.shape
+    rows, V = logits.shape
+    _need(scores, torch.float32, (B, W), "scores")
+    if rows != B * W or logits.stride(1) != 1:
+        raise ValueError(f"logits must be {B * W} rows of contiguous values")
+    if out is None:
+        out = (torch.empty((B, topk), dtype=torch.float32, device=dev),
+               torch.empty((B, topk), dtype=torch.int32, device=dev),
+               torch.empty((B, topk), dtype=torch.int32, device=dev))
+    else:
+        for t, dt, name in zip(out, (torch.float32, torch.int32, torch.int32),
+                               ("score", "beam", "token")):
+            _need(t, dt, (B, topk), name)
+    if workspace is None:
+        workspace = BeamWorkspace(B, W, V, topk, dev)
+    if any(t.device != dev for t in (scores, workspace.buffer) + tuple(out)):
+        raise ValueError("logits, scores, workspace and out must be on one device")
+    st = abi.lib().pvlc_lm_head_beam_topk(
+        logits.data_ptr(), int(logits.dtype == torch.float16),
+        logits.stride(0) if rows > 1 else max(V, logits.stride(0)), scores.data_ptr(), B, W, V,
+        topk, workspace.buffer.data_ptr(), workspace.nbytes, out[0].data_ptr(),
+        out[1].data_ptr(), out[2].data_ptr(), torch.cuda.current_stream().cuda_stream)
+    abi.check(st, "pvlc_lm_head_beam_topk")
+    return tuple(out)
