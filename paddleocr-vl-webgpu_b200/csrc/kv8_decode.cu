@@ -7,17 +7,54 @@
 // (fp16); a tail that is now full is quantised into page table[slot][n / 32].
 //   s_r = scale_K(r) (q . k_r) / sqrt(128),   out = sum_r softmax(s)_r scale_V(r) v_r
 //
+// The scales never touch a matrix operand.  scale_K multiplies the f32 scores
+// of a page.  scale_V goes into the exponent: with t_r = s_r log2(e) +
+// log2(scale_V(r)) and M the running maximum of t,
+//   w_r = 2^(t_r - M + 14)   (fp16, at most 2^14, kept down to 2^-24: 2^-38 of the largest)
+//   O = sum_r w_r code_r,    L = sum_r w_r / scale_V(r),    out = O / L,
+// so the codes go to the tensor cores as the fp16 numbers they are.
+//
+// Bound by HBM: 2 x 128 bytes a row and KV head, 16 operations a byte at a
+// group of 8.  What the design does about it:
+//   * The (sequence, KV head) units, each its pages and a tail, are laid end to
+//     end with an allowance for a unit's end, and cut into equal ranges, one per
+//     block and two blocks per SM, whatever the lengths are.
+//   * A producer warp streams pages (4 KB of K and of V codes, one TMA tile
+//     each, 128-byte swizzle) through a ring of 8 KB stages; it looks 32 pages
+//     ahead in the table.  A page's scales follow by cp.async on the same barrier.
+//   * Four consumer warps take the pages in turn, each with its own running
+//     (O, M, L), so they meet only at a unit's end.
+//   * S^T = K Q^T and O^T += V^T W^T with mma.m16n8k16: the 8 query heads of a
+//     group are the N side (two N tiles above 8).  The contraction order is
+//     free, so a lane's 16-byte loads are whole operand fragments: 16 dims of a
+//     key row, and 16 dims of four value rows whose bytes are paired with prmt.
+//     Keys are permuted by pi(g) = g / 2 + 4 (g % 2) within 8 and value dims by
+//     the same map of 16-dim chunks, which makes every load conflict free.
+//   * A unit that spans blocks leaves a partial record per block; the last one to
+//     finish joins them in block order.
+//
 // The rotation multiplies and adds with a rounding each (no fused
 // multiply-add), so a cached key row is the plain f32 formula's, bit for bit.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <mutex>
+
 #include "kv8.cuh"
+#include "tcgen05.cuh"
 
 namespace pvlc {
 namespace kv8 {
 
-constexpr int MAX_GROUP = 16;
+constexpr int WARPS = 4;                          // consumer warps
+constexpr int THREADS = (WARPS + 1) * 32;
+constexpr int CTHREADS = WARPS * 32;
+constexpr uint32_t STAGE = 8192;                  // a page's K and V codes of one head
+constexpr uint32_t END_COST = 3;                  // a unit's end, in pages
+constexpr uint32_t MIN_COST = 8;                  // least work of a block, in pages
+constexpr int ACC_PITCH = HD + 4;
+constexpr float W_SHIFT = 14.f;
 
 struct DecodeParams {
   View c;
@@ -29,11 +66,13 @@ struct DecodeParams {
   const int32_t* rope_row;
   const int32_t* slot;
   __half* out;
-  uint32_t q_stride, kv_stride, rope_rows, batch, group;
+  uint32_t q_stride, kv_stride, rope_rows, batch, group, stages;
   uint32_t* flags;
+  uint32_t* tickets;
+  float* records;
 };
 
-// What is wrong with sequence b (0: nothing); its slot, rows and table row.
+// What is wrong with sequence b (0: nothing); its rows and rope row.
 __device__ __forceinline__ uint32_t check_sequence(const DecodeParams& p, uint32_t b, int32_t slot,
                                                    int32_t* rows, uint32_t* rope) {
   if (slot < 0 || (uint32_t)slot >= p.c.slots) return kFlagSlot;
@@ -47,126 +86,732 @@ __device__ __forceinline__ uint32_t check_sequence(const DecodeParams& p, uint32
   return bad;
 }
 
-// Dim d of a head row rotated: x cos - y sin below 64 (y = dim d + 64),
-// x cos + y sin above (y = dim d - 64).
-__device__ __forceinline__ float rotated(const __half* row, uint32_t d, const DecodeParams& p,
-                                         uint32_t r) {
-  const size_t at = ((size_t)mrope_axis(d) * p.rope_rows + r) * HD + d;
-  const float x = __half2float(row[d]), y = __half2float(row[d ^ 64]);
-  return __fadd_rn(__fmul_rn(x, p.rope_cos[at]), __fmul_rn(d < 64 ? -y : y, p.rope_sin[at]));
+// 16 dims d .. d + 15 (d a multiple of 16, below 64) and their partners 64
+// above, rotated: lo cos - hi sin, hi cos + lo sin; as fp16 pairs.
+__device__ __forceinline__ void rotate16(const __half* row, uint32_t d, const DecodeParams& p,
+                                         uint32_t r, uint32_t* lo_out, uint32_t* hi_out) {
+#pragma unroll
+  for (int e = 0; e < 16; e += 4) {
+    const uint2 lw = __ldg(reinterpret_cast<const uint2*>(row + d + e));
+    const uint2 hw = __ldg(reinterpret_cast<const uint2*>(row + d + 64 + e));
+    const size_t at = ((size_t)mrope_axis(d + e) * p.rope_rows + r) * HD + d + e;
+    const float4 cl = __ldg(reinterpret_cast<const float4*>(p.rope_cos + at));
+    const float4 ch = __ldg(reinterpret_cast<const float4*>(p.rope_cos + at + 64));
+    const float4 sl = __ldg(reinterpret_cast<const float4*>(p.rope_sin + at));
+    const float4 sh = __ldg(reinterpret_cast<const float4*>(p.rope_sin + at + 64));
+    const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&lw.x));
+    const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&lw.y));
+    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hw.x));
+    const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hw.y));
+    auto turn = [](float x, float c, float y, float s) {
+      return __fadd_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+    };
+    lo_out[e / 2] = pack_half2(turn(l0.x, cl.x, -h0.x, sl.x), turn(l0.y, cl.y, -h0.y, sl.y));
+    lo_out[e / 2 + 1] = pack_half2(turn(l1.x, cl.z, -h1.x, sl.z), turn(l1.y, cl.w, -h1.y, sl.w));
+    hi_out[e / 2] = pack_half2(turn(h0.x, ch.x, l0.x, sh.x), turn(h0.y, ch.y, l0.y, sh.y));
+    hi_out[e / 2 + 1] = pack_half2(turn(h1.x, ch.z, l1.x, sh.z), turn(h1.y, ch.w, l1.y, sh.w));
+  }
 }
 
-// One block per (KV head, sequence), thread d = dim d.
+// The low / high two code bytes of a word as an fp16 pair (exact).
 template <int CODE>
-__global__ void __launch_bounds__(HD) kv8_decode_kernel(const DecodeParams p) {
-  __shared__ float q[MAX_GROUP][HD];
-  __shared__ float w[MAX_GROUP][PAGE];
-  __shared__ float m[MAX_GROUP], l[MAX_GROUP], f[MAX_GROUP];
-  const uint32_t h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const int warp = d >> 5, lane = d & 31;
-  const int32_t slot = p.slot ? p.slot[b] : (int32_t)b;
-  if (slot == -1) return;
-  const uint32_t G = p.group, QH = G * p.c.heads;
-  __half* out = p.out + ((size_t)b * QH + h * G) * HD;
-  int32_t n = 0;
-  uint32_t rr = 0;
-  if (const uint32_t bad = check_sequence(p, b, slot, &n, &rr)) {
-    if (d == 0) atomicOr(p.flags, bad);
-    for (uint32_t i = 0; i < G; ++i) out[i * HD + d] = __float2half_rn(0.f);
-    return;
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+  if (CODE == PVLC_KV8_E4M3) {
+    uint32_t d;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(w));
+    return d;
   }
-  const __half* qr = p.q + (size_t)b * p.q_stride + (size_t)h * G * HD;
-  for (uint32_t i = 0; i < G; ++i)
-    q[i][d] = __half2float(__float2half_rn(rotated(qr + i * HD, d, p, rr))) * 0.08838834764831845f;
-  __half* tk = tail_rows(p.c, slot, 0, h);
-  __half* tv = tail_rows(p.c, slot, 1, h);
-  const uint32_t last = n % PAGE, full = n / PAGE;
-  tk[last * HD + d] = __float2half_rn(rotated(p.k_new + (size_t)b * p.kv_stride + h * HD, d, p, rr));
-  tv[last * HD + d] = p.v_new[(size_t)b * p.kv_stride + h * HD + d];
-  if (d < G) {
-    m[d] = -CUDART_INF_F;
-    l[d] = 0.f;
+  // 0x6400 | u is 1024 + u for a byte u; u = code + 128
+  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140);
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1152.f));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <int CODE>
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  if (CODE == PVLC_KV8_E4M3) {
+    uint32_t d;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(d) : "r"(w));
+    return d;
   }
-  float o[MAX_GROUP];
-  for (uint32_t i = 0; i < MAX_GROUP; ++i) o[i] = 0.f;
-  __syncthreads();
-  const int32_t* row = p.c.table + (size_t)slot * p.c.max_pages;
-  for (uint32_t j = 0; j <= full; ++j) {
-    const bool open = j == full;
-    const uint32_t live = open ? last + 1 : PAGE;
-    const uint8_t *kc = nullptr, *vc = nullptr;
-    float sk = 1.f, sv = 1.f;
-    if (!open) {
-      const int32_t page = row[j];
-      if (page < 0 || (uint32_t)page >= p.c.pages) {
-        if (d == 0) atomicOr(p.flags, kFlagPage);
-        sk = sv = CUDART_NAN_F;
-        kc = vc = p.c.codes;
-      } else {
-        kc = block_codes(p.c, page, 0, h);
-        vc = block_codes(p.c, page, 1, h);
-        sk = p.c.scales[((size_t)page * p.c.heads + h) * 2];
-        sv = p.c.scales[((size_t)page * p.c.heads + h) * 2 + 1];
+  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1152.f));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// A loaded word of codes as codes_lo / codes_hi take it.
+template <int CODE>
+__device__ __forceinline__ uint32_t biased(uint32_t w) {
+  return CODE == PVLC_KV8_E4M3 ? w : w ^ 0x80808080u;
+}
+
+// A consumer warp's state over one unit: O^T tiles (tile i: dims 16 chunk +
+// 2 i and + 2 i + 1 on fragment rows g and g + 8; heads 2 t, 2 t + 1), the
+// running maximum and this lane's share of L, per head.
+template <int NT>
+struct Acc {
+  float o[NT][8][4];
+  float m[NT][2], l[NT][2];
+};
+
+// Scores of 32 keys (fragment row g of half tile mt is key 16 mt + pi(g), g + 8
+// eight above) into weights, with the running maximum; `live` keys count.
+template <int NT>
+__device__ __forceinline__ void weigh(float (&s)[2][NT][4], Acc<NT>& a, float kk, float lsv,
+                                      float rsv, int key0, int live, uint32_t (&w)[2][NT][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float t0 = -CUDART_INF_F, t1 = -CUDART_INF_F;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float* x = s[mt][nt] + 2 * r;
+        const bool on = key0 + 16 * mt + 8 * r < live;
+        x[0] = on ? x[0] * kk + lsv : -CUDART_INF_F;
+        x[1] = on ? x[1] * kk + lsv : -CUDART_INF_F;
+        t0 = fmaxf(t0, x[0]);
+        t1 = fmaxf(t1, x[1]);
+      }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+      t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+    }
+    if (__any_sync(0xffffffffu, t0 > a.m[nt][0] || t1 > a.m[nt][1])) {
+      const float m0 = fmaxf(a.m[nt][0], t0), m1 = fmaxf(a.m[nt][1], t1);
+      const float f0 = fast_exp2(a.m[nt][0] - m0), f1 = fast_exp2(a.m[nt][1] - m1);
+      a.m[nt][0] = m0;
+      a.m[nt][1] = m1;
+      a.l[nt][0] *= f0;
+      a.l[nt][1] *= f1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a.o[nt][i][0] *= f0;
+        a.o[nt][i][1] *= f1;
+        a.o[nt][i][2] *= f0;
+        a.o[nt][i][3] *= f1;
       }
     }
-    auto value = [&](const uint8_t* codes, const __half* tail, uint32_t r, uint32_t e) {
-      if (open) return __half2float(tail[r * HD + e]);
-      if (CODE == PVLC_KV8_INT8) return (float)(int8_t)codes[r * HD + e];
-      return __half2float(__half(__nv_cvt_fp8_to_halfraw(codes[r * HD + e], __NV_E4M3)));
-    };
-    for (uint32_t r = warp; r < live; r += HD / 32)
-      for (uint32_t i = 0; i < G; ++i) {
-        float s = 0.f;
-        for (uint32_t e = lane; e < HD; e += 32) s += q[i][e] * value(kc, tk, r, e);
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        if (lane == 0) w[i][r] = s * sk;
+    const float c0 = W_SHIFT - a.m[nt][0], c1 = W_SHIFT - a.m[nt][1];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float p0 = fast_exp2(s[mt][nt][2 * r] + c0), p1 = fast_exp2(s[mt][nt][2 * r + 1] + c1);
+        a.l[nt][0] += p0 * rsv;
+        a.l[nt][1] += p1 * rsv;
+        w[mt][nt][r] = movmatrix_t(pack_half2(p0, p1));
       }
-    __syncthreads();
-    for (uint32_t i = warp; i < G; i += HD / 32) {
-      const float s = lane < live ? w[i][lane] : -CUDART_INF_F;
-      float top = fmaxf(m[i], s);
-      for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float e = lane < live ? expf(s - top) : 0.f;
-      float sum = e;
-      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      w[i][lane] = e * sv;
-      __syncwarp();
-      if (lane == 0) {
-        f[i] = expf(m[i] - top);
-        l[i] = l[i] * f[i] + sum;
-        m[i] = top;
-      }
-    }
-    __syncthreads();
-    for (uint32_t i = 0; i < G; ++i) {
-      float s = o[i] * f[i];
-      for (uint32_t r = 0; r < live; ++r) s += w[i][r] * value(vc, tv, r, d);
-      o[i] = s;
-    }
-    __syncthreads();
   }
-  for (uint32_t i = 0; i < G; ++i) out[i * HD + d] = __float2half_rn(o[i] / l[i]);
-  if (last == PAGE - 1 && warp < 2) {   // the block is full: warp 0 its keys, warp 1 its values
-    const int32_t page = row[full];
-    if (page < 0 || (uint32_t)page >= p.c.pages) {
-      if (lane == 0) atomicOr(p.flags, kFlagPage);
-      return;
+}
+
+// One page of codes at `st` (K, then V 4 KB above, both swizzled).
+template <int CODE, int NT>
+__device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv, float qk,
+                                          const uint32_t (&qf)[NT][16], Acc<NT>& a, int g, int t) {
+  const int pi = (g >> 1) | ((g & 1) << 2);
+  float s[2][NT][4];
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint8_t* at = st + (16 * mt + pi) * HD + (((t + 4 * j) ^ pi) << 4);
+      const uint4 xa = *reinterpret_cast<const uint4*>(at);
+      const uint4 xb = *reinterpret_cast<const uint4*>(at + 8 * HD);
+      const uint32_t wa[4] = {xa.x, xa.y, xa.z, xa.w}, wb[4] = {xb.x, xb.y, xb.z, xb.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t ya = biased<CODE>(wa[e]), yb = biased<CODE>(wb[e]);
+        const uint32_t a0 = codes_lo<CODE>(ya), a1 = codes_lo<CODE>(yb);
+        const uint32_t a2 = codes_hi<CODE>(ya), a3 = codes_hi<CODE>(yb);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma_16816(s[mt][nt], a0, a1, a2, a3, qf[nt][8 * j + 2 * e], qf[nt][8 * j + 2 * e + 1]);
+      }
     }
-    const uint4* x4 = reinterpret_cast<const uint4*>(warp ? tv : tk);
-    uint4 x[16];
+  }
+  uint32_t w[2][NT][2];
+  weigh<NT>(s, a, sk * qk, __log2f(sv), __frcp_rn(sv), 0, 64, w);
+  // value rows t, t + 4, t + 8, t + 12 of a half tile: keys pi(2 t), pi(2 t + 1), ..
+  const uint8_t* v = st + 4096;
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+    uint32_t x[4][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * mt + t + 4 * r;
+      const uint4 y = *reinterpret_cast<const uint4*>(v + row * HD + ((pi ^ (row & 7)) << 4));
+      x[r][0] = biased<CODE>(y.x);
+      x[r][1] = biased<CODE>(y.y);
+      x[r][2] = biased<CODE>(y.z);
+      x[r][3] = biased<CODE>(y.w);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[2 * i] = x4[(4 * i + (lane >> 3)) * (HD / 8) + 2 * (lane & 7)];
-      x[2 * i + 1] = x4[(4 * i + (lane >> 3)) * (HD / 8) + 2 * (lane & 7) + 1];
+      const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+      const uint32_t y0 = __byte_perm(x[0][i >> 1], x[1][i >> 1], sel);
+      const uint32_t y1 = __byte_perm(x[2][i >> 1], x[3][i >> 1], sel);
+      const uint32_t a0 = codes_lo<CODE>(y0), a1 = codes_hi<CODE>(y0);
+      const uint32_t a2 = codes_lo<CODE>(y1), a3 = codes_hi<CODE>(y1);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        mma_16816(a.o[nt][i], a0, a1, a2, a3, w[mt][nt][0], w[mt][nt][1]);
     }
-    quantise_block<CODE>(x, block_codes(p.c, page, warp, h),
-                         p.c.scales + ((size_t)page * p.c.heads + h) * 2 + warp, lane);
   }
+}
+
+// The open block: fp16 rows 0 .. last - 1 at kt, vt and row `last` at kn, vn.
+template <int NT>
+__device__ __forceinline__ void tail_tile(const uint8_t* kt, const uint8_t* vt, const uint8_t* kn,
+                                          const uint8_t* vn, int last, float qk,
+                                          const uint32_t (&qf)[NT][16], Acc<NT>& a, int g, int t) {
+  const int pi = (g >> 1) | ((g & 1) << 2);
+  float s[2][NT][4];
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+    const int ra = 16 * mt + pi, rb = ra + 8;
+    const uint8_t* pa = ra < last ? kt + ra * 256 : kn;
+    const uint8_t* pb = rb < last ? kt + rb * 256 : kn;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const uint4 xa = *reinterpret_cast<const uint4*>(pa + (t + 4 * j) * 32 + 16 * f);
+        const uint4 xb = *reinterpret_cast<const uint4*>(pb + (t + 4 * j) * 32 + 16 * f);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint32_t* qq = qf[nt] + 8 * j + 4 * f;
+          mma_16816(s[mt][nt], xa.x, xb.x, xa.y, xb.y, qq[0], qq[1]);
+          mma_16816(s[mt][nt], xa.z, xb.z, xa.w, xb.w, qq[2], qq[3]);
+        }
+      }
+  }
+  uint32_t w[2][NT][2];
+  weigh<NT>(s, a, qk, 0.f, 1.f, pi, last + 1, w);
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      uint32_t x[4][4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * mt + t + 4 * r;
+        const uint8_t* at = row < last ? vt + row * 256 : vn;
+        uint4 y = *reinterpret_cast<const uint4*>(at + pi * 32 + 16 * f);
+        if (row > last) y = make_uint4(0, 0, 0, 0);
+        x[r][0] = y.x;
+        x[r][1] = y.y;
+        x[r][2] = y.z;
+        x[r][3] = y.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t a0 = __byte_perm(x[0][e], x[1][e], 0x5410);
+        const uint32_t a1 = __byte_perm(x[0][e], x[1][e], 0x7632);
+        const uint32_t a2 = __byte_perm(x[2][e], x[3][e], 0x5410);
+        const uint32_t a3 = __byte_perm(x[2][e], x[3][e], 0x7632);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma_16816(a.o[nt][4 * f + e], a0, a1, a2, a3, w[mt][nt][0], w[mt][nt][1]);
+      }
+    }
+  }
+}
+
+// The block whose cost range holds position y of a line of C cut into G.
+__device__ __forceinline__ uint32_t owner_of(uint64_t y, uint64_t G, uint64_t C) {
+  return static_cast<uint32_t>(((y + 1) * G + C - 1) / C - 1);
+}
+
+struct Seq {
+  uint32_t cost;     // cost position of the sequence's first unit, per KV head
+  int32_t slot, rows;
+  uint32_t rope;
+};
+
+template <int NT>
+constexpr uint32_t record_floats() { return 8 * NT * (HD + 2); }
+template <int NT>
+constexpr uint32_t fixed_smem() {
+  return WARPS * 8 * NT * (ACC_PITCH + 2) * 4 + WARPS * 512 + 64;
+}
+
+template <int CODE, int NT>
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
+    kv8_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap map) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  // ring | unit ends [WARPS][8 NT] rows, maxima, sums | new rows [WARPS][2][256 B] | sequences |
+  // scales and barriers of the stages
+  const uint32_t S = p.stages, B = p.batch, H = p.c.heads, G = p.group;
+  uint8_t* ring = smem;
+  float* end_acc = reinterpret_cast<float*>(smem + S * STAGE);
+  float* end_m = end_acc + WARPS * 8 * NT * ACC_PITCH;
+  float* end_l = end_m + WARPS * 8 * NT;
+  uint8_t* fresh = reinterpret_cast<uint8_t*>(end_l + WARPS * 8 * NT);
+  uint32_t* misc = reinterpret_cast<uint32_t*>(fresh + WARPS * 512);   // [16]
+  Seq* seq = reinterpret_cast<Seq*>(misc + 16);                        // [B + 1]
+  float2* scale = reinterpret_cast<float2*>(seq + B + 1);              // [S]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scale + S);             // [S]
+  uint64_t* empty = full + S;                                          // [S]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (uint32_t i = 0; i < S; ++i) {
+      mbar_init(full + i, 2);
+      mbar_init(empty + i, 1);
+    }
+    fence_mbar_init();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- the line of costs: pages + 1 + END_COST for each valid sequence and head
+  {
+    const uint32_t per = (B + THREADS - 1) / THREADS;
+    const uint32_t b0 = min(B, tid * per), b1 = min(B, b0 + per);
+    uint32_t sum = 0;
+    for (uint32_t b = b0; b < b1; ++b) {
+      Seq s;
+      s.slot = p.slot ? p.slot[b] : (int32_t)b;
+      s.rows = 0;
+      s.rope = 0;
+      s.cost = sum;
+      uint32_t bad = 0;
+      if (s.slot != -1) bad = check_sequence(p, b, s.slot, &s.rows, &s.rope);
+      if (bad) {
+        s.slot = -1;
+        if (b % gridDim.x == blockIdx.x) {
+          atomicOr(p.flags, bad);
+          uint4* o = reinterpret_cast<uint4*>(p.out + (size_t)b * G * H * HD);
+          for (uint32_t i = 0; i < G * H * HD / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (s.slot >= 0) sum += s.rows / PAGE + 1 + END_COST;
+      seq[b] = s;
+    }
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) misc[warp] = incl;
+    __syncthreads();
+    uint32_t before = incl - sum;
+    for (int i = 0; i < warp; ++i) before += misc[i];
+    for (uint32_t b = b0; b < b1; ++b) seq[b].cost += before;
+    if (tid == THREADS - 1) seq[B].cost = before + sum;
+    __syncthreads();
+  }
+  const uint64_t C = (uint64_t)seq[B].cost * H;
+  if (C == 0) return;
+  const uint64_t N = umax64(1, umin64(gridDim.x, C / MIN_COST));
+  if (blockIdx.x >= N) return;
+  const uint64_t y0 = blockIdx.x * C / N, y1 = (blockIdx.x + 1) * C / N;
+  // the last sequence whose line starts at or before y (idle ones have no length)
+  auto seq_at = [&](uint64_t y) -> uint32_t {
+    uint32_t lo = 0, hi = B;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if ((uint64_t)seq[mid].cost * H <= y) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+
+  if (warp == WARPS) {
+    // ============================ producer ============================
+    uint32_t stage = 0, phase = 0, issued = 0;
+    bool alive = true;
+    auto claim = [&]() {              // the next stage is free (the lanes agree)
+      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(empty + stage, phase ^ 1));
+      return alive;
+    };
+    auto next = [&]() {
+      ++issued;
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
+      }
+    };
+    // position y of the line: page >= 0, -1: nothing, -2: a tail (packed in x),
+    // -3: a page id out of range
+    struct Item {
+      int32_t kind;
+      uint32_t b, h;
+    };
+    auto look = [&](uint64_t y) {
+      Item it{-1, 0, 0};
+      if (y < y1) {
+        it.b = seq_at(y);
+        const Seq s = seq[it.b];
+        const uint32_t np = s.rows / PAGE, len = np + 1 + END_COST;
+        const uint32_t u = (uint32_t)(y - (uint64_t)s.cost * H);
+        it.h = u / len;
+        const uint32_t i = u % len;
+        if (i < np) {
+          const int32_t page = p.c.table[(size_t)s.slot * p.c.max_pages + i];
+          it.kind = page >= 0 && (uint32_t)page < p.c.pages ? page : -3;
+        } else if (i == np) {
+          it.kind = -2;
+        }
+      }
+      return it;
+    };
+    Item ahead = look(y0 + lane);
+    for (uint64_t y = y0; y < y1 && alive; y += 32) {
+      const Item now = ahead;
+      ahead = look(y + 32 + lane);
+      const int n = (int)umin64(32, y1 - y);
+      for (int e = 0; e < n && alive; ++e) {
+        const int32_t kind = __shfl_sync(0xffffffffu, now.kind, e);
+        const uint32_t h = __shfl_sync(0xffffffffu, now.h, e);
+        if (kind == -1) continue;
+        const uint32_t b = __shfl_sync(0xffffffffu, now.b, e);
+        if (!claim()) break;
+        if (kind == -2) {
+          // the tail's rows before the append: K in one stage, V in the next
+          const uint32_t bytes = seq[b].rows % PAGE * 256;
+          for (uint32_t kv = 0; kv < 2; ++kv) {
+            if (kv && !claim()) break;
+            if (lane == 0) {
+              mbar_arrive(full + stage);
+              if (bytes) {
+                mbar_arrive_expect_tx(full + stage, bytes);
+                bulk_g2s(ring + stage * STAGE, tail_rows(p.c, seq[b].slot, kv, h), bytes,
+                         full + stage);
+              } else {
+                mbar_arrive(full + stage);
+              }
+            }
+            next();
+          }
+        } else {
+          if (lane == 0) {
+            if (kind == -3) {
+              atomicOr(p.flags, kFlagPage);
+              scale[stage] = make_float2(CUDART_NAN_F, CUDART_NAN_F);
+              mbar_arrive(full + stage);
+              mbar_arrive(full + stage);
+            } else {
+              mbar_arrive_expect_tx(full + stage, STAGE);
+              const int32_t row = (int32_t)(((uint32_t)kind * 2 * H + h) * PAGE);
+              tc::tma_load_2d(ring + stage * STAGE, &map, 0, row, full + stage);
+              tc::tma_load_2d(ring + stage * STAGE + 4096, &map, 0, row + (int32_t)(H * PAGE), full + stage);
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(scale + stage)),
+                           "l"(p.c.scales + ((size_t)kind * H + h) * 2)
+                           : "memory");
+              cp_async_arrive_noinc(full + stage);
+            }
+          }
+          next();
+        }
+      }
+    }
+    if (!alive && lane == 0) atomicOr(p.flags, kFlagTimeout);   // a stage was not freed in time
+    // leave no copy in flight, whatever the consumers did
+    const uint32_t n = min(issued, S);
+    for (uint32_t i = 0; i < n; ++i) {
+      if (stage == 0) {
+        stage = S;
+        phase ^= 1;
+      }
+      --stage;
+      mbar_wait(full + stage, phase);
+    }
+    cp_async_wait_all();
+    return;
+  }
+
+  // ============================= consumers ============================
+  const int g = lane >> 2, t = lane & 3;
+  const float qk = 1.4426950408889634f * 0.08838834764831845f;   // log2(e) / sqrt(128)
+  uint8_t* my_fresh = fresh + warp * 512;
+  uint32_t stage = 0, phase = 0;      // of ring position `at`
+  uint32_t at = 0;                    // ring position of the segment's first item
+  uint32_t turn = 0;                  // items before this segment, modulo WARPS
+  bool alive = true;
+  uint32_t seen = 0;                  // ring position of (stage, phase)
+  auto seek = [&](uint32_t k) {
+    for (; seen < k; ++seen)
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
+      }
+  };
+  auto arrived = [&]() {              // the current stage's data
+    if (alive) {
+      alive = __all_sync(0xffffffffu, mbar_wait(full + stage, phase));
+      if (!alive && lane == 0) atomicOr(p.flags, kFlagTimeout);
+    }
+    return alive;
+  };
+  // A warp that gave up frees no more stages, so the producer gives up too; it
+  // goes on to meet the other warps at the unit ends.
+  auto release = [&](uint32_t s) {
+    __syncwarp();
+    if (alive && lane == 0) mbar_arrive(empty + s);
+  };
+
+  uint32_t b = seq_at(y0);
+  uint32_t h;
+  {
+    const uint32_t len = seq[b].rows / PAGE + 1 + END_COST;
+    h = (uint32_t)((y0 - (uint64_t)seq[b].cost * H) / len);
+  }
+  while (true) {
+    const Seq sq = seq[b];
+    const uint32_t np = sq.rows / PAGE, len = np + 1 + END_COST;
+    const uint64_t u0 = (uint64_t)sq.cost * H + (uint64_t)h * len;
+    if (u0 >= y1) break;
+    const uint32_t i0 = (uint32_t)(umax64(y0, u0) - u0);
+    const uint32_t i1 = min((uint32_t)(umin64(y1, u0 + len) - u0), np + 1);
+    if (i0 < i1) {
+      // ---------------------------------------------- this block's pages
+      Acc<NT> a;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a.o[nt][i][e] = 0.f;
+        a.m[nt][0] = a.m[nt][1] = -CUDART_INF_F;
+        a.l[nt][0] = a.l[nt][1] = 0.f;
+      }
+      const uint32_t first = (warp + WARPS - turn) % WARPS;     // this warp's first item
+      if (i0 + first < i1) {
+        uint32_t qf[NT][16];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (nt * 8 + g < (int)G) {
+            rotate16(p.q + (size_t)b * p.q_stride + ((size_t)h * G + nt * 8 + g) * HD, 16 * t, p,
+                     sq.rope, qf[nt], qf[nt] + 8);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) qf[nt][e] = 0;
+          }
+        }
+        for (uint32_t i = i0 + first; i < i1; i += WARPS) {
+          seek(at + i - i0);
+          if (i < np) {
+            if (arrived()) {
+              const float2 sc = scale[stage];
+              page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, a, g, t);
+            }
+            release(stage);
+            continue;
+          }
+          // ------------------------------------------------ append and tail
+          const int last = sq.rows % PAGE;
+          uint4* kn = reinterpret_cast<uint4*>(my_fresh);
+          uint4* vn = kn + 16;
+          __half* tk = tail_rows(p.c, sq.slot, 0, h);
+          __half* tv = tail_rows(p.c, sq.slot, 1, h);
+          if (lane < 4) {
+            uint32_t lo[8], hi[8];
+            rotate16(p.k_new + (size_t)b * p.kv_stride + h * HD, 16 * lane, p, sq.rope, lo, hi);
+            uint4* row = reinterpret_cast<uint4*>(tk + last * HD);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint4 x = make_uint4(lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]);
+              const uint4 y = make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
+              row[2 * lane + e] = kn[2 * lane + e] = x;
+              row[8 + 2 * lane + e] = kn[8 + 2 * lane + e] = y;
+            }
+          } else if (lane >= 16) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(
+                                      p.v_new + (size_t)b * p.kv_stride + h * HD) + lane - 16);
+            reinterpret_cast<uint4*>(tv + last * HD)[lane - 16] = vn[lane - 16] = x;
+          }
+          __syncwarp();
+          const uint32_t s0 = stage;
+          arrived();
+          const uint8_t* kt = ring + stage * STAGE;
+          seek(at + i - i0 + 1);
+          arrived();
+          const uint8_t* vt = ring + stage * STAGE;
+          if (alive) {
+            tail_tile<NT>(kt, vt, my_fresh, my_fresh + 256, last, qk, qf, a, g, t);
+            if (last == PAGE - 1) {            // the block is full
+              const int32_t page = p.c.table[(size_t)sq.slot * p.c.max_pages + np];
+              if (page < 0 || (uint32_t)page >= p.c.pages) {
+                if (lane == 0) atomicOr(p.flags, kFlagPage);
+              } else {
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv) {
+                  uint4 x[16];
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    const int r = 4 * e + (lane >> 3);
+                    const uint8_t* row = r < last ? (kv ? vt : kt) + r * 256 : my_fresh + kv * 256;
+                    x[2 * e] = *reinterpret_cast<const uint4*>(row + (lane & 7) * 32);
+                    x[2 * e + 1] = *reinterpret_cast<const uint4*>(row + (lane & 7) * 32 + 16);
+                  }
+                  quantise_block<CODE>(x, block_codes(p.c, page, kv, h),
+                                       p.c.scales + ((size_t)page * H + h) * 2 + kv, lane);
+                }
+              }
+            }
+          }
+          release(stage);
+          release(s0);
+        }
+      }
+      at += i1 - i0 + (i1 == np + 1 ? 1 : 0);
+      turn = (turn + i1 - i0) % WARPS;
+      // ------------------------------------------------- join the warps
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float l = a.l[nt][c];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          const int head = warp * 8 * NT + nt * 8 + 2 * t + c;
+          if (g == 0) {
+            end_m[head] = a.m[nt][c];
+            end_l[head] = l;
+          }
+          float* row = end_acc + head * ACC_PITCH + 16 * ((g >> 1) | ((g & 1) << 2));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(row + 4 * k) =
+                make_float4(a.o[nt][2 * k][c], a.o[nt][2 * k][c + 2], a.o[nt][2 * k + 1][c],
+                            a.o[nt][2 * k + 1][c + 2]);
+        }
+      }
+      named_bar_sync(1, CTHREADS);
+      const bool whole = i0 == 0 && i1 == np + 1;
+      float* rec = p.records + (size_t)(blockIdx.x * 2 + (u0 >= y0 ? 1 : 0)) * record_floats<NT>();
+      __half* out = p.out + ((size_t)b * H + h) * G * HD + tid;
+      for (uint32_t i = 0; i < G; ++i) {
+        float m = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, end_m[w * 8 * NT + i]);
+        float o = 0.f, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const int head = w * 8 * NT + i;
+          // a warp without pages has maximum -inf and adds nothing
+          const float f = end_l[head] == 0.f ? 0.f : fast_exp2(end_m[head] - m);
+          o += end_acc[head * ACC_PITCH + tid] * f;
+          l += end_l[head] * f;
+        }
+        if (whole) {
+          out[i * HD] = __float2half_rn(o / l);
+        } else {
+          rec[i * HD + tid] = o;
+          if (tid == 0) {
+            rec[8 * NT * HD + i] = m;
+            rec[8 * NT * (HD + 1) + i] = l;
+          }
+        }
+      }
+      if (!whole) {
+        // ------------------------------------------- join the blocks
+        __threadfence();
+        named_bar_sync(1, CTHREADS);
+        const uint32_t c0 = owner_of(u0, N, C), c1 = owner_of(u0 + np, N, C);
+        if (tid == 0) {
+          uint32_t* ticket = p.tickets + b * H + h;
+          const uint32_t before = atomicAdd(ticket, 1);
+          const bool mine = before == c1 - c0;
+          if (mine) *ticket = 0;
+          misc[8] = mine;
+        }
+        named_bar_sync(1, CTHREADS);
+        if (misc[8]) {
+          __threadfence();
+          auto record = [&](uint32_t c) {
+            const bool starts = c == c0 && u0 >= (uint64_t)c * C / N;
+            return p.records + (size_t)(c * 2 + (starts ? 1 : 0)) * record_floats<NT>();
+          };
+          for (uint32_t i = 0; i < G; ++i) {
+            float m = -CUDART_INF_F;
+            for (uint32_t c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(record(c) + 8 * NT * HD + i));
+            float o = 0.f, l = 0.f;
+            for (uint32_t c = c0; c <= c1; ++c) {
+              const float* r = record(c);
+              const float f = fast_exp2(__ldcg(r + 8 * NT * HD + i) - m);
+              l += __ldcg(r + 8 * NT * (HD + 1) + i) * f;
+              o += __ldcg(r + i * HD + tid) * f;
+            }
+            out[i * HD] = __float2half_rn(o / l);
+          }
+        }
+      }
+      named_bar_sync(1, CTHREADS);     // the unit's buffers have been read
+    }
+    if (++h == H) {
+      h = 0;
+      do ++b; while (b < B && seq[b].slot < 0);
+      if (b == B) break;
+    }
+  }
+}
+
+// ------------------------------------------------------------------- host
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(ptr);
+  });
+  return fn;
+}
+
+// Two blocks on an SM with one N tile; with two, one block of up to 255 registers a thread.
+template <int NT>
+constexpr uint32_t block_smem() { return NT == 1 ? 112 * 1024 : 224 * 1024; }
+
+template <int CODE, int NT>
+int decode_variant(DecodeParams& p, const CUtensorMap& map, uint64_t most_cost, int sms,
+                   cudaStream_t stream) {
+  const uint32_t fixed = fixed_smem<NT>() + (p.batch + 1) * sizeof(Seq);
+  const uint32_t per = STAGE + 8 + 16;
+  p.stages = (block_smem<NT>() - fixed) / per;
+  const uint32_t bytes = fixed + p.stages * per;
+  const void* fn = reinterpret_cast<const void*>(kv8_decode_kernel<CODE, NT>);
+  if (const int st = set_smem_attribute_once(fn, block_smem<NT>())) return st;
+  const uint64_t blocks = most_cost / MIN_COST, room = (NT == 1 ? 2 : 1) * (uint64_t)sms;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((uint32_t)(blocks < 1 ? 1 : blocks < room ? blocks : room));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv8_decode_kernel<CODE, NT>, p, map) == cudaSuccess
+             ? PVLC_OK
+             : PVLC_CUDA_ERROR;
 }
 
 }  // namespace kv8
 
-size_t kv8_decode_scratch_bytes(uint32_t, uint32_t, uint32_t) { return 0; }
+size_t kv8_decode_scratch_bytes(uint32_t, uint32_t query_heads, uint32_t kv_heads) {
+  const bool wide = query_heads / kv_heads > 8;
+  return (size_t)sms_or_default_count() * 2 * 2 * 4 *
+         (wide ? kv8::record_floats<2>() : kv8::record_floats<1>());
+}
 
 int kv8_decode_launch(const pvlc_kv8_cache& c, uint32_t layer, const Kv8DecodeArgs& a,
                       cudaStream_t stream) {
@@ -185,13 +830,31 @@ int kv8_decode_launch(const pvlc_kv8_cache& c, uint32_t layer, const Kv8DecodeAr
   p.rope_rows = a.rope_rows;
   p.batch = a.batch;
   p.group = a.query_heads / c.kv_heads;
+  p.stages = 0;
   p.flags = static_cast<uint32_t*>(a.workspace);
-  const dim3 grid(c.kv_heads, a.batch);
-  if (c.code_type == PVLC_KV8_E4M3)
-    kv8::kv8_decode_kernel<PVLC_KV8_E4M3><<<grid, kv8::HD, 0, stream>>>(p);
-  else
-    kv8::kv8_decode_kernel<PVLC_KV8_INT8><<<grid, kv8::HD, 0, stream>>>(p);
-  return cudaPeekAtLastError() == cudaSuccess ? PVLC_OK : PVLC_CUDA_ERROR;
+  p.tickets = kv8_tickets(a.workspace);
+  p.records = reinterpret_cast<float*>(kv8_scratch(a.workspace));
+  const int sms = device_sm_count();
+  if (sms <= 0) return PVLC_CUDA_ERROR;
+  kv8::EncodeTiled enc = kv8::encoder();
+  if (!enc) return PVLC_CUDA_ERROR;
+  // a layer's codes as 128-byte rows; a box is one (page, K or V, head) block
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {128, (cuuint64_t)c.pages * 2 * c.kv_heads * kv8::PAGE};
+  const cuuint64_t strides[1] = {128};
+  const cuuint32_t box[2] = {128, kv8::PAGE};
+  const cuuint32_t estr[2] = {1, 1};
+  if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.c.codes, dims, strides, box, estr,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return PVLC_CUDA_ERROR;
+  const uint64_t most = (uint64_t)a.batch * c.kv_heads * (c.max_pages + 1 + kv8::END_COST);
+  const bool e4m3 = c.code_type == PVLC_KV8_E4M3;
+  if (p.group > 8)
+    return e4m3 ? kv8::decode_variant<PVLC_KV8_E4M3, 2>(p, map, most, sms, stream)
+                : kv8::decode_variant<PVLC_KV8_INT8, 2>(p, map, most, sms, stream);
+  return e4m3 ? kv8::decode_variant<PVLC_KV8_E4M3, 1>(p, map, most, sms, stream)
+              : kv8::decode_variant<PVLC_KV8_INT8, 1>(p, map, most, sms, stream);
 }
 
 }  // namespace pvlc
