@@ -47,8 +47,11 @@
 namespace pvlc {
 namespace kv8 {
 
-constexpr int WARPS = 4;                          // consumer warps
-constexpr int THREADS = (WARPS + 1) * 32;
+#ifndef KV8_WARPS
+#define KV8_WARPS 4
+#endif
+constexpr int WARPS = KV8_WARPS;                  // consumer warps
+constexpr int THREADS = (WARPS + 2) * 32;         // + the producer and the sequence warp
 constexpr int CTHREADS = WARPS * 32;
 constexpr uint32_t STAGE = 8192;                  // a page's K and V codes of one head
 constexpr uint32_t END_COST = 3;                  // a unit's end, in pages
@@ -338,24 +341,139 @@ struct Seq {
 
 template <int NT>
 constexpr uint32_t record_floats() { return 8 * NT * (HD + 2); }
+// acc += f x[0 .. 8)
+__device__ __forceinline__ void add_scaled(float (&acc)[8], const float* x, float f) {
+  const float4 a = *reinterpret_cast<const float4*>(x), b = *reinterpret_cast<const float4*>(x + 4);
+  acc[0] += a.x * f;
+  acc[1] += a.y * f;
+  acc[2] += a.z * f;
+  acc[3] += a.w * f;
+  acc[4] += b.x * f;
+  acc[5] += b.y * f;
+  acc[6] += b.z * f;
+  acc[7] += b.w * f;
+}
+__device__ __forceinline__ void write_out(__half* out, const float (&o)[8], float l) {
+  const float r = 1.f / l;
+  *reinterpret_cast<uint4*>(out) =
+      make_uint4(pack_half2(o[0] * r, o[1] * r), pack_half2(o[2] * r, o[3] * r),
+                 pack_half2(o[4] * r, o[5] * r), pack_half2(o[6] * r, o[7] * r));
+}
+
+// The output of a unit from its n blocks' records, in block order: half a warp
+// takes a head, lane `sub` of it dims 8 sub .. + 7 and every 16th record's
+// maximum and sum.  A group of 8 records is read with independent loads.
+template <int NT>
+__device__ __forceinline__ void join_blocks(const float* records, uint32_t r0, uint32_t n,
+                                            uint32_t G, __half* out, int warp, int lane) {
+  const uint32_t sub = lane & 15;
+  auto record = [&](uint32_t c) {
+    // record r0 is block c0's second or only one; the others are their blocks' first
+    return records + (size_t)(c == 0 ? r0 : (r0 & ~1u) + 2 * c) * record_floats<NT>();
+  };
+  for (uint32_t i0 = 2 * warp; i0 < G; i0 += 2 * WARPS) {
+    const uint32_t i = i0 + (lane >> 4);
+    const uint32_t ii = i < G ? i : 0;           // the lanes stay together
+    float m = -CUDART_INF_F;
+    for (uint32_t c = sub; c < n; c += 16) m = fmaxf(m, __ldcg(record(c) + 8 * NT * HD + ii));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (uint32_t base = 0; base < n; base += 8) {
+      float4 x[8][2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (base + e < n) {
+          const float4* r = reinterpret_cast<const float4*>(record(base + e) + ii * HD + 8 * sub);
+          x[e][0] = __ldcg(r);
+          x[e][1] = __ldcg(r + 1);
+        }
+      float f = 0.f, fl = 0.f;
+      if (sub < 8 && base + sub < n) {
+        const float* r = record(base + sub) + 8 * NT * HD + ii;
+        f = fast_exp2(__ldcg(r) - m);
+        fl = __ldcg(r + 8 * NT) * f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float fe = __shfl_sync(0xffffffffu, f, e, 16);
+        l += __shfl_sync(0xffffffffu, fl, e, 16);
+        if (base + e < n) {
+          o[0] += x[e][0].x * fe;
+          o[1] += x[e][0].y * fe;
+          o[2] += x[e][0].z * fe;
+          o[3] += x[e][0].w * fe;
+          o[4] += x[e][1].x * fe;
+          o[5] += x[e][1].y * fe;
+          o[6] += x[e][1].z * fe;
+          o[7] += x[e][1].w * fe;
+        }
+      }
+    }
+    if (i < G) write_out(out + i * HD + 8 * sub, o, l);
+  }
+}
+
+// The units of a block's range [y0, y1): sequence b, KV head h, whose items
+// [i0, i1) of np pages and a tail (item np) are the block's.
+struct Units {
+  const Seq* seq;
+  uint32_t B, H, b, h, np, i0, i1;
+  uint64_t y0, y1, u0;
+  Seq sq;
+  __device__ __forceinline__ Units(const Seq* seq_, uint32_t B_, uint32_t H_, uint64_t y0_,
+                                   uint64_t y1_, uint32_t b_)
+      : seq(seq_), B(B_), H(H_), b(b_), y0(y0_), y1(y1_) {
+    const uint32_t len = seq[b].rows / PAGE + 1 + END_COST;
+    h = (uint32_t)((y0 - (uint64_t)seq[b].cost * H) / len);
+    set();
+  }
+  __device__ __forceinline__ void set() {
+    sq = seq[b];
+    np = sq.rows / PAGE;
+    const uint32_t len = np + 1 + END_COST;
+    u0 = (uint64_t)sq.cost * H + (uint64_t)h * len;
+    i0 = u0 < y0 ? (uint32_t)(y0 - u0) : 0;
+    i1 = u0 < y1 ? min((uint32_t)umin64(y1 - u0, len), np + 1) : 0;
+  }
+  __device__ __forceinline__ bool valid() const { return b < B && u0 < y1; }
+  __device__ __forceinline__ bool has_pages() const { return i0 < i1; }
+  __device__ __forceinline__ bool has_tail() const { return i1 == np + 1; }
+  __device__ __forceinline__ void step() {
+    if (++h == H) {
+      h = 0;
+      do ++b; while (b < B && seq[b].slot < 0);
+    }
+    if (b < B) set();
+  }
+};
+
+// A unit's rotated q as the consumers' fragments [NT][4][32 lanes] x 16 bytes, then its new
+// key and value rows.
+template <int NT>
+constexpr uint32_t seq_slot() { return NT * 2048 + 512; }
+
 template <int NT>
 constexpr uint32_t fixed_smem() {
-  return WARPS * 8 * NT * (ACC_PITCH + 2) * 4 + WARPS * 512 + 64;
+  return WARPS * 8 * NT * (ACC_PITCH + 2) * 4 + 2 * seq_slot<NT>() + 64 + 64;
 }
 
 template <int CODE, int NT>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     kv8_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap map) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  // ring | unit ends [WARPS][8 NT] rows, maxima, sums | new rows [WARPS][2][256 B] | sequences |
-  // scales and barriers of the stages
+  // ring | unit ends [WARPS][8 NT] rows, maxima, sums | two unit slots | sequences | scales and
+  // barriers of the stages
   const uint32_t S = p.stages, B = p.batch, H = p.c.heads, G = p.group;
   uint8_t* ring = smem;
   float* end_acc = reinterpret_cast<float*>(smem + S * STAGE);
   float* end_m = end_acc + WARPS * 8 * NT * ACC_PITCH;
   float* end_l = end_m + WARPS * 8 * NT;
-  uint8_t* fresh = reinterpret_cast<uint8_t*>(end_l + WARPS * 8 * NT);
-  uint32_t* misc = reinterpret_cast<uint32_t*>(fresh + WARPS * 512);   // [16]
+  uint8_t* slots = reinterpret_cast<uint8_t*>(end_l + WARPS * 8 * NT);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(slots + 2 * seq_slot<NT>());   // [2]
+  uint64_t* row_full = q_full + 2;                                     // [2]
+  uint64_t* slot_empty = row_full + 2;                                 // [2]
+  uint32_t* misc = reinterpret_cast<uint32_t*>(q_full + 8);            // [16]
   Seq* seq = reinterpret_cast<Seq*>(misc + 16);                        // [B + 1]
   float2* scale = reinterpret_cast<float2*>(seq + B + 1);              // [S]
   uint64_t* full = reinterpret_cast<uint64_t*>(scale + S);             // [S]
@@ -366,6 +484,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     for (uint32_t i = 0; i < S; ++i) {
       mbar_init(full + i, 2);
       mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 32);
+      mbar_init(row_full + i, 32);
+      mbar_init(slot_empty + i, WARPS);
+      misc[8 + 4 * i] = 0;
     }
     fence_mbar_init();
   }
@@ -529,10 +653,71 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     return;
   }
 
+  if (warp == WARPS + 1) {
+    // ========================= sequence warp ========================
+    // Per unit of this block, up to two ahead of the consumers: the rotated q
+    // into the unit's slot, then, where the block holds the unit's tail, the
+    // rotated key and the value into the slot and into the tail (the append).
+    Units it(seq, B, H, y0, y1, seq_at(y0));
+    uint32_t n = 0;
+    for (; it.valid(); it.step()) {
+      if (!it.has_pages()) continue;
+      const uint32_t s = n & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(slot_empty + s, (n >> 1 & 1) ^ 1))) {
+        if (lane == 0) atomicOr(p.flags, kFlagTimeout);
+        return;
+      }
+      uint8_t* slot = slots + s * seq_slot<NT>();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t w[16];
+        const uint32_t head = nt * 8 + (lane >> 2);
+        if (head < G) {
+          rotate16(p.q + (size_t)it.b * p.q_stride + ((size_t)it.h * G + head) * HD,
+                   16 * (lane & 3), p, it.sq.rope, w, w + 8);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          reinterpret_cast<uint4*>(slot)[(nt * 4 + e) * 32 + lane] =
+              make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+      }
+      mbar_arrive(q_full + s);
+      if (it.has_tail()) {
+        const int last = it.sq.rows % PAGE;
+        uint4* kn = reinterpret_cast<uint4*>(slot + NT * 2048);
+        uint4* vn = kn + 16;
+        if (lane < 4) {
+          uint32_t w[16];
+          rotate16(p.k_new + (size_t)it.b * p.kv_stride + it.h * HD, 16 * lane, p, it.sq.rope, w,
+                   w + 8);
+          uint4* row = reinterpret_cast<uint4*>(tail_rows(p.c, it.sq.slot, 0, it.h) + last * HD);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint4 x = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+            const int at = (e & 2) * 4 + 2 * lane + (e & 1);
+            row[at] = x;
+            kn[at] = x;
+          }
+        } else if (lane >= 16) {
+          const uint4 x = __ldg(reinterpret_cast<const uint4*>(
+                                    p.v_new + (size_t)it.b * p.kv_stride + it.h * HD) + lane - 16);
+          reinterpret_cast<uint4*>(tail_rows(p.c, it.sq.slot, 1, it.h) + last * HD)[lane - 16] = x;
+          vn[lane - 16] = x;
+        }
+        __syncwarp();
+      }
+      mbar_arrive(row_full + s);
+      ++n;
+    }
+    return;
+  }
+
   // ============================= consumers ============================
   const int g = lane >> 2, t = lane & 3;
   const float qk = 1.4426950408889634f * 0.08838834764831845f;   // log2(e) / sqrt(128)
-  uint8_t* my_fresh = fresh + warp * 512;
   uint32_t stage = 0, phase = 0;      // of ring position `at`
   uint32_t at = 0;                    // ring position of the segment's first item
   uint32_t turn = 0;                  // items before this segment, modulo WARPS
@@ -545,9 +730,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         phase ^= 1;
       }
   };
-  auto arrived = [&]() {              // the current stage's data
+  auto arrived = [&](uint64_t* bar, uint32_t parity) {
     if (alive) {
-      alive = __all_sync(0xffffffffu, mbar_wait(full + stage, phase));
+      alive = __all_sync(0xffffffffu, mbar_wait(bar, parity));
       if (!alive && lane == 0) atomicOr(p.flags, kFlagTimeout);
     }
     return alive;
@@ -559,20 +744,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     if (alive && lane == 0) mbar_arrive(empty + s);
   };
 
-  uint32_t b = seq_at(y0);
-  uint32_t h;
-  {
-    const uint32_t len = seq[b].rows / PAGE + 1 + END_COST;
-    h = (uint32_t)((y0 - (uint64_t)seq[b].cost * H) / len);
-  }
-  while (true) {
-    const Seq sq = seq[b];
-    const uint32_t np = sq.rows / PAGE, len = np + 1 + END_COST;
-    const uint64_t u0 = (uint64_t)sq.cost * H + (uint64_t)h * len;
-    if (u0 >= y1) break;
-    const uint32_t i0 = (uint32_t)(umax64(y0, u0) - u0);
-    const uint32_t i1 = min((uint32_t)(umin64(y1, u0 + len) - u0), np + 1);
-    if (i0 < i1) {
+  uint32_t unit = 0;                  // units of this block so far
+  for (Units it(seq, B, H, y0, y1, seq_at(y0)); it.valid(); it.step()) {
+    const Seq sq = it.sq;
+    const uint32_t b = it.b, h = it.h, np = it.np, i0 = it.i0, i1 = it.i1;
+    const uint64_t u0 = it.u0;
+    if (it.has_pages()) {
       // ---------------------------------------------- this block's pages
       Acc<NT> a;
 #pragma unroll
@@ -585,84 +762,51 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         a.l[nt][0] = a.l[nt][1] = 0.f;
       }
       const uint32_t first = (warp + WARPS - turn) % WARPS;     // this warp's first item
-      if (i0 + first < i1) {
+      const uint8_t* slot = slots + (unit & 1) * seq_slot<NT>();
+      const uint32_t slot_phase = unit >> 1 & 1;
+      if (i0 + first < i1 && arrived(q_full + (unit & 1), slot_phase)) {
         uint32_t qf[NT][16];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (nt * 8 + g < (int)G) {
-            rotate16(p.q + (size_t)b * p.q_stride + ((size_t)h * G + nt * 8 + g) * HD, 16 * t, p,
-                     sq.rope, qf[nt], qf[nt] + 8);
-          } else {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) qf[nt][e] = 0;
+          for (int e = 0; e < 4; ++e) {
+            const uint4 x = reinterpret_cast<const uint4*>(slot)[(nt * 4 + e) * 32 + lane];
+            qf[nt][4 * e] = x.x;
+            qf[nt][4 * e + 1] = x.y;
+            qf[nt][4 * e + 2] = x.z;
+            qf[nt][4 * e + 3] = x.w;
           }
-        }
         for (uint32_t i = i0 + first; i < i1; i += WARPS) {
           seek(at + i - i0);
           if (i < np) {
-            if (arrived()) {
+            if (arrived(full + stage, phase)) {
               const float2 sc = scale[stage];
               page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, a, g, t);
             }
             release(stage);
             continue;
           }
-          // ------------------------------------------------ append and tail
+          // ----------------------------------------------------------- tail
           const int last = sq.rows % PAGE;
-          uint4* kn = reinterpret_cast<uint4*>(my_fresh);
-          uint4* vn = kn + 16;
-          __half* tk = tail_rows(p.c, sq.slot, 0, h);
-          __half* tv = tail_rows(p.c, sq.slot, 1, h);
-          if (lane < 4) {
-            uint32_t lo[8], hi[8];
-            rotate16(p.k_new + (size_t)b * p.kv_stride + h * HD, 16 * lane, p, sq.rope, lo, hi);
-            uint4* row = reinterpret_cast<uint4*>(tk + last * HD);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint4 x = make_uint4(lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]);
-              const uint4 y = make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
-              row[2 * lane + e] = kn[2 * lane + e] = x;
-              row[8 + 2 * lane + e] = kn[8 + 2 * lane + e] = y;
-            }
-          } else if (lane >= 16) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4*>(
-                                      p.v_new + (size_t)b * p.kv_stride + h * HD) + lane - 16);
-            reinterpret_cast<uint4*>(tv + last * HD)[lane - 16] = vn[lane - 16] = x;
-          }
-          __syncwarp();
+          const uint8_t* rows = slot + NT * 2048;
           const uint32_t s0 = stage;
-          arrived();
+          arrived(full + stage, phase);
           const uint8_t* kt = ring + stage * STAGE;
           seek(at + i - i0 + 1);
-          arrived();
+          arrived(full + stage, phase);
           const uint8_t* vt = ring + stage * STAGE;
-          if (alive) {
-            tail_tile<NT>(kt, vt, my_fresh, my_fresh + 256, last, qk, qf, a, g, t);
-            if (last == PAGE - 1) {            // the block is full
-              const int32_t page = p.c.table[(size_t)sq.slot * p.c.max_pages + np];
-              if (page < 0 || (uint32_t)page >= p.c.pages) {
-                if (lane == 0) atomicOr(p.flags, kFlagPage);
-              } else {
-#pragma unroll 1
-                for (int kv = 0; kv < 2; ++kv) {
-                  uint4 x[16];
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) {
-                    const int r = 4 * e + (lane >> 3);
-                    const uint8_t* row = r < last ? (kv ? vt : kt) + r * 256 : my_fresh + kv * 256;
-                    x[2 * e] = *reinterpret_cast<const uint4*>(row + (lane & 7) * 32);
-                    x[2 * e + 1] = *reinterpret_cast<const uint4*>(row + (lane & 7) * 32 + 16);
-                  }
-                  quantise_block<CODE>(x, block_codes(p.c, page, kv, h),
-                                       p.c.scales + ((size_t)page * H + h) * 2 + kv, lane);
-                }
-              }
-            }
+          if (arrived(row_full + (unit & 1), slot_phase)) {
+            tail_tile<NT>(kt, vt, rows, rows + 256, last, qk, qf, a, g, t);
           }
           release(stage);
           release(s0);
         }
       }
+      // the row barrier advances with the slot, also past warps that do not use it
+      arrived(row_full + (unit & 1), slot_phase);
+      __syncwarp();
+      if (alive && lane == 0) mbar_arrive(slot_empty + (unit & 1));
+      ++unit;
       at += i1 - i0 + (i1 == np + 1 ? 1 : 0);
       turn = (turn + i1 - i0) % WARPS;
       // ------------------------------------------------- join the warps
@@ -687,72 +831,84 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         }
       }
       named_bar_sync(1, CTHREADS);
+      // half a warp takes a head, each lane 8 of its dims
       const bool whole = i0 == 0 && i1 == np + 1;
       float* rec = p.records + (size_t)(blockIdx.x * 2 + (u0 >= y0 ? 1 : 0)) * record_floats<NT>();
-      __half* out = p.out + ((size_t)b * H + h) * G * HD + tid;
-      for (uint32_t i = 0; i < G; ++i) {
-        float m = -CUDART_INF_F;
+      __half* out = p.out + ((size_t)b * H + h) * G * HD;
+      const uint32_t sub = lane & 15;
+      for (uint32_t i = 2 * warp + (lane >> 4); i < G; i += 2 * WARPS) {
+        float m = -CUDART_INF_F, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) m = fmaxf(m, end_m[w * 8 * NT + i]);
-        float o = 0.f, l = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
           const int head = w * 8 * NT + i;
+          const float wl = end_l[head];
           // a warp without pages has maximum -inf and adds nothing
-          const float f = end_l[head] == 0.f ? 0.f : fast_exp2(end_m[head] - m);
-          o += end_acc[head * ACC_PITCH + tid] * f;
-          l += end_l[head] * f;
+          const float f = wl == 0.f ? 0.f : fast_exp2(end_m[head] - m);
+          l += wl * f;
+          add_scaled(o, end_acc + head * ACC_PITCH + 8 * sub, f);
         }
         if (whole) {
-          out[i * HD] = __float2half_rn(o / l);
+          write_out(out + i * HD + 8 * sub, o, l);
         } else {
-          rec[i * HD + tid] = o;
-          if (tid == 0) {
+          float4* to = reinterpret_cast<float4*>(rec + i * HD + 8 * sub);
+          to[0] = make_float4(o[0], o[1], o[2], o[3]);
+          to[1] = make_float4(o[4], o[5], o[6], o[7]);
+          if (sub == 0) {
             rec[8 * NT * HD + i] = m;
             rec[8 * NT * (HD + 1) + i] = l;
           }
         }
       }
-      if (!whole) {
-        // ------------------------------------------- join the blocks
-        __threadfence();
-        named_bar_sync(1, CTHREADS);
-        const uint32_t c0 = owner_of(u0, N, C), c1 = owner_of(u0 + np, N, C);
-        if (tid == 0) {
-          uint32_t* ticket = p.tickets + b * H + h;
-          const uint32_t before = atomicAdd(ticket, 1);
-          const bool mine = before == c1 - c0;
-          if (mine) *ticket = 0;
-          misc[8] = mine;
-        }
-        named_bar_sync(1, CTHREADS);
-        if (misc[8]) {
-          __threadfence();
-          auto record = [&](uint32_t c) {
-            const bool starts = c == c0 && u0 >= (uint64_t)c * C / N;
-            return p.records + (size_t)(c * 2 + (starts ? 1 : 0)) * record_floats<NT>();
-          };
-          for (uint32_t i = 0; i < G; ++i) {
-            float m = -CUDART_INF_F;
-            for (uint32_t c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(record(c) + 8 * NT * HD + i));
-            float o = 0.f, l = 0.f;
-            for (uint32_t c = c0; c <= c1; ++c) {
-              const float* r = record(c);
-              const float f = fast_exp2(__ldcg(r + 8 * NT * HD + i) - m);
-              l += __ldcg(r + 8 * NT * (HD + 1) + i) * f;
-              o += __ldcg(r + i * HD + tid) * f;
-            }
-            out[i * HD] = __float2half_rn(o / l);
-          }
+      if (!whole && tid == 0) {         // joined when the block is through
+        uint32_t* e = misc + 8 + (u0 >= y0 ? 4 : 0);
+        e[0] = 1;
+        e[1] = b;
+        e[2] = h;
+      }
+      if (it.has_tail() && sq.rows % PAGE == PAGE - 1 && warp < 2) {
+        // the open block is full: warp 0 quantises its keys, warp 1 its values
+        const int32_t page = p.c.table[(size_t)sq.slot * p.c.max_pages + np];
+        if (page < 0 || (uint32_t)page >= p.c.pages) {
+          if (lane == 0) atomicOr(p.flags, kFlagPage);
+        } else {
+          const uint4* from = reinterpret_cast<const uint4*>(tail_rows(p.c, sq.slot, warp, h));
+          uint4 x[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            x[e] = from[(e >> 1) * 64 + (lane >> 3) * 16 + (lane & 7) * 2 + (e & 1)];
+          quantise_block<CODE>(x, block_codes(p.c, page, warp, h),
+                               p.c.scales + ((size_t)page * H + h) * 2 + warp, lane);
         }
       }
       named_bar_sync(1, CTHREADS);     // the unit's buffers have been read
     }
-    if (++h == H) {
-      h = 0;
-      do ++b; while (b < B && seq[b].slot < 0);
-      if (b == B) break;
-    }
+  }
+
+  // -------------------------------------------------- join the blocks
+  // At most two units span blocks: one that began in an earlier block (its
+  // record is this block's first) and one that goes on in a later block.
+  __threadfence();
+  named_bar_sync(1, CTHREADS);
+  if (tid < 2 && misc[8 + 4 * tid]) {
+    const uint32_t b = misc[9 + 4 * tid], h = misc[10 + 4 * tid];
+    const uint32_t np = seq[b].rows / PAGE;
+    const uint64_t u0 = (uint64_t)seq[b].cost * H + (uint64_t)h * (np + 1 + END_COST);
+    const uint32_t c0 = owner_of(u0, N, C), c1 = owner_of(u0 + np, N, C);
+    uint32_t* ticket = p.tickets + b * H + h;
+    const bool mine = atomicAdd(ticket, 1) == c1 - c0;
+    if (mine) *ticket = 0;
+    misc[8 + 4 * tid] = mine ? c1 - c0 + 1 : 0;
+    misc[11 + 4 * tid] = c0 * 2 + (u0 >= (uint64_t)c0 * C / N ? 1 : 0);   // block c0's record
+  }
+  named_bar_sync(1, CTHREADS);
+  for (int s = 0; s < 2; ++s) {
+    const uint32_t n = misc[8 + 4 * s];
+    if (n == 0) continue;
+    __threadfence();
+    join_blocks<NT>(p.records, misc[11 + 4 * s], n, G,
+                    p.out + ((size_t)misc[9 + 4 * s] * H + misc[10 + 4 * s]) * G * HD, warp, lane);
   }
 }
 
