@@ -737,6 +737,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     }
     return alive;
   };
+  // The current stage's data.  Copies may land out of order, so a warp may get
+  // here before the stage's previous page (another warp's) has even landed, when
+  // the full barrier is a phase behind and its parity says the wrong thing.  So
+  // it waits for that page to be freed first: the empty barrier is never more
+  // than a phase behind, because a position less than S - 1 earlier has been seen.
+  auto landed = [&]() {
+    return arrived(empty + stage, phase ^ 1) && arrived(full + stage, phase);
+  };
   // A warp that gave up frees no more stages, so the producer gives up too; it
   // goes on to meet the other warps at the unit ends.
   auto release = [&](uint32_t s) {
@@ -779,7 +787,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         for (uint32_t i = i0 + first; i < i1; i += WARPS) {
           seek(at + i - i0);
           if (i < np) {
-            if (arrived(full + stage, phase)) {
+            if (landed()) {
               const float2 sc = scale[stage];
               page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, a, g, t);
             }
@@ -790,10 +798,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           const int last = sq.rows % PAGE;
           const uint8_t* rows = slot + NT * 2048;
           const uint32_t s0 = stage;
-          arrived(full + stage, phase);
+          landed();
           const uint8_t* kt = ring + stage * STAGE;
           seek(at + i - i0 + 1);
-          arrived(full + stage, phase);
+          landed();
           const uint8_t* vt = ring + stage * STAGE;
           if (arrived(row_full + (unit & 1), slot_phase)) {
             tail_tile<NT>(kt, vt, rows, rows + 256, last, qk, qf, a, g, t);
@@ -940,8 +948,12 @@ template <int CODE, int NT>
 int decode_variant(DecodeParams& p, const CUtensorMap& map, uint64_t most_cost, int sms,
                    cudaStream_t stream) {
   const uint32_t fixed = fixed_smem<NT>() + (p.batch + 1) * sizeof(Seq);
-  const uint32_t per = STAGE + 8 + 16;
+  constexpr uint32_t per = STAGE + 8 + 16;
   p.stages = (block_smem<NT>() - fixed) / per;
+  // a warp's items are at most WARPS + 1 ring positions apart
+  static_assert((block_smem<NT>() - fixed_smem<NT>() - (PVLC_KV8_MAX_BATCH + 1) * sizeof(Seq)) / per >=
+                    WARPS + 2,
+                "too few ring stages");
   const uint32_t bytes = fixed + p.stages * per;
   const void* fn = reinterpret_cast<const void*>(kv8_decode_kernel<CODE, NT>);
   if (const int st = set_smem_attribute_once(fn, block_smem<NT>())) return st;
