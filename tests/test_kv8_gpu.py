@@ -577,7 +577,7 @@ def test_wrapper_refusals(kv8):
         kv8.Cache(c.codes, c.scales, c.tails[:, :1], c.table, c.tokens, c.refs)
     with pytest.raises(TypeError):
         kv8.Cache(c.codes.view(torch.uint8), c.scales, c.tails, c.table, c.tokens, c.refs)
-    small = kv8.Workspace(kv8.Cache.empty(1, 4, 2, 4, 2), 1, 16)
-    big = kv8.Cache.empty(1, 100000, 2, 4, 1)
+    small = kv8.Workspace(c, 2, 16)
+    small.nbytes = 4096
     with pytest.raises(abi.PvlcError):
-        kv8.grow(big, slot, small, ahead=1)
+        kv8.grow(c, slot, small, ahead=1)
