@@ -551,104 +551,90 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
 
   if (warp == WARPS) {
     // ============================ producer ============================
-    uint32_t stage = 0, phase = 0, issued = 0;
-    bool alive = true;
-    auto claim = [&]() {              // the next stage is free (the lanes agree)
-      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(empty + stage, phase ^ 1));
-      return alive;
-    };
-    auto next = [&]() {
-      ++issued;
-      if (++stage == S) {
-        stage = 0;
-        phase ^= 1;
-      }
-    };
-    // position y of the line: page >= 0, -1: nothing, -2: a tail (packed in x),
-    // -3: a page id out of range
-    struct Item {
-      int32_t kind;
-      uint32_t b, h;
-    };
-    auto look = [&](uint64_t y) {
-      Item it{-1, 0, 0};
-      if (y < y1) {
-        it.b = seq_at(y);
-        const Seq s = seq[it.b];
-        const uint32_t np = s.rows / PAGE, len = np + 1 + END_COST;
-        const uint32_t u = (uint32_t)(y - (uint64_t)s.cost * H);
-        it.h = u / len;
-        const uint32_t i = u % len;
-        if (i < np) {
-          const int32_t page = p.c.table[(size_t)s.slot * p.c.max_pages + i];
-          it.kind = page >= 0 && (uint32_t)page < p.c.pages ? page : -3;
-        } else if (i == np) {
-          it.kind = -2;
-        }
-      }
-      return it;
-    };
-    Item ahead = look(y0 + lane);
-    for (uint64_t y = y0; y < y1 && alive; y += 32) {
-      const Item now = ahead;
-      ahead = look(y + 32 + lane);
-      const int n = (int)umin64(32, y1 - y);
-      for (int e = 0; e < n && alive; ++e) {
-        const int32_t kind = __shfl_sync(0xffffffffu, now.kind, e);
-        const uint32_t h = __shfl_sync(0xffffffffu, now.h, e);
-        if (kind == -1) continue;
-        const uint32_t b = __shfl_sync(0xffffffffu, now.b, e);
-        if (!claim()) break;
-        if (kind == -2) {
-          // the tail's rows before the append: K in one stage, V in the next
-          const uint32_t bytes = seq[b].rows % PAGE * 256;
-          for (uint32_t kv = 0; kv < 2; ++kv) {
-            if (kv && !claim()) break;
-            if (lane == 0) {
-              mbar_arrive(full + stage);
-              if (bytes) {
-                mbar_arrive_expect_tx(full + stage, bytes);
-                bulk_g2s(ring + stage * STAGE, tail_rows(p.c, seq[b].slot, kv, h), bytes,
-                         full + stage);
-              } else {
-                mbar_arrive(full + stage);
-              }
-            }
-            next();
+    // Lane l feeds stage l: ring positions l, l + S, .. of the block's items.
+    // It walks the units by itself and loads its next page's id while it waits
+    // for the stage, so one pass of the loop serves every stage that is free, in
+    // ring order (the consumers' waits rely on it).
+    Units it(seq, B, H, y0, y1, seq_at(y0));
+    uint32_t base = 0;                // ring position of the unit's first item
+    int32_t page = -1;                // >= 0: a page; -1: an id out of range; -2, -3: K, V tail
+    auto find = [&](uint32_t k) {     // the item of ring position k; false behind the last
+      while (it.valid()) {
+        const uint32_t n = it.has_pages() ? it.i1 - it.i0 + (it.has_tail() ? 1 : 0) : 0;
+        if (k < base + n) {
+          const uint32_t i = it.i0 + (k - base);
+          if (i >= it.np) {
+            page = -2 - (int32_t)(i - it.np);
+          } else {
+            page = p.c.table[(size_t)it.sq.slot * p.c.max_pages + i];
+            if (page < 0 || (uint32_t)page >= p.c.pages) page = -1;
           }
+          return true;
+        }
+        base += n;
+        it.step();
+      }
+      return false;
+    };
+    uint32_t k = lane, phase = 0;
+    bool more = lane < (int)S && find(k);
+    uint64_t* my_full = full + lane;
+    uint8_t* st = ring + lane * STAGE;
+    uint32_t head = 0, head_stage = 0;   // the first position not issued, the same in all lanes
+    uint32_t idle = 0;
+    uint64_t since = 0;
+    while (__any_sync(0xffffffffu, more)) {
+      const uint64_t ready =
+          __ballot_sync(0xffffffffu, more && mbar_try_wait(empty + lane, phase ^ 1));
+      // stages ready in a row from the head's on
+      const uint64_t row = (ready | ready << S) >> head_stage;
+      const uint32_t n = min(S, (uint32_t)__ffsll((long long)~row) - 1);
+      if (more && k - head < n) {
+        if (page >= 0) {
+          mbar_arrive_expect_tx(my_full, STAGE);
+          const int32_t row = (int32_t)(((uint32_t)page * 2 * H + it.h) * PAGE);
+          tc::tma_load_2d(st, &map, 0, row, my_full);
+          tc::tma_load_2d(st + 4096, &map, 0, row + (int32_t)(H * PAGE), my_full);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(scale + lane)),
+                       "l"(p.c.scales + ((size_t)page * H + it.h) * 2)
+                       : "memory");
+          cp_async_arrive_noinc(my_full);
+        } else if (page == -1) {
+          atomicOr(p.flags, kFlagPage);
+          scale[lane] = make_float2(CUDART_NAN_F, CUDART_NAN_F);
+          mbar_arrive(my_full);
+          mbar_arrive(my_full);
         } else {
-          if (lane == 0) {
-            if (kind == -3) {
-              atomicOr(p.flags, kFlagPage);
-              scale[stage] = make_float2(CUDART_NAN_F, CUDART_NAN_F);
-              mbar_arrive(full + stage);
-              mbar_arrive(full + stage);
-            } else {
-              mbar_arrive_expect_tx(full + stage, STAGE);
-              const int32_t row = (int32_t)(((uint32_t)kind * 2 * H + h) * PAGE);
-              tc::tma_load_2d(ring + stage * STAGE, &map, 0, row, full + stage);
-              tc::tma_load_2d(ring + stage * STAGE + 4096, &map, 0, row + (int32_t)(H * PAGE), full + stage);
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(scale + stage)),
-                           "l"(p.c.scales + ((size_t)kind * H + h) * 2)
-                           : "memory");
-              cp_async_arrive_noinc(full + stage);
-            }
+          // the tail's rows before the append
+          const uint32_t bytes = it.sq.rows % PAGE * 256;
+          mbar_arrive(my_full);
+          if (bytes) {
+            mbar_arrive_expect_tx(my_full, bytes);
+            bulk_g2s(st, tail_rows(p.c, it.sq.slot, -2 - page, it.h), bytes, my_full);
+          } else {
+            mbar_arrive(my_full);
           }
-          next();
+        }
+        phase ^= 1;
+        k += S;
+        more = find(k);
+      }
+      head += n;
+      head_stage += n;
+      if (head_stage >= S) head_stage -= S;
+      if (n) {
+        idle = 0;
+      } else if (++idle >= 64) {      // nothing was free for a while: bound the wait
+        const uint64_t now = globaltimer();
+        if (idle == 64) since = now;
+        if (__any_sync(0xffffffffu, now - since > kWaitLimitNs)) {
+          if (lane == 0) atomicOr(p.flags, kFlagTimeout);
+          break;
         }
       }
     }
-    if (!alive && lane == 0) atomicOr(p.flags, kFlagTimeout);   // a stage was not freed in time
     // leave no copy in flight, whatever the consumers did
-    const uint32_t n = min(issued, S);
-    for (uint32_t i = 0; i < n; ++i) {
-      if (stage == 0) {
-        stage = S;
-        phase ^= 1;
-      }
-      --stage;
-      mbar_wait(full + stage, phase);
-    }
+    if (lane < (int)S && k >= S) mbar_wait(my_full, phase ^ 1);
     cp_async_wait_all();
     return;
   }
@@ -718,17 +704,18 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   // ============================= consumers ============================
   const int g = lane >> 2, t = lane & 3;
   const float qk = 1.4426950408889634f * 0.08838834764831845f;   // log2(e) / sqrt(128)
-  uint32_t stage = 0, phase = 0;      // of ring position `at`
-  uint32_t at = 0;                    // ring position of the segment's first item
-  uint32_t turn = 0;                  // items before this segment, modulo WARPS
+  uint32_t at = 0;                    // ring position of the unit's first item
+  uint32_t turn = 0;                  // items before this unit, modulo WARPS
   bool alive = true;
-  uint32_t seen = 0;                  // ring position of (stage, phase)
-  auto seek = [&](uint32_t k) {
-    for (; seen < k; ++seen)
-      if (++stage == S) {
-        stage = 0;
-        phase ^= 1;
-      }
+  uint32_t stage = 0, phase = 0;      // of ring position `seen`
+  uint32_t seen = 0;
+  auto seek = [&](uint32_t k) {       // less than two rounds ahead
+    stage += k - seen;
+    seen = k;
+    while (stage >= S) {
+      stage -= S;
+      phase ^= 1;
+    }
   };
   auto arrived = [&](uint64_t* bar, uint32_t parity) {
     if (alive) {
@@ -950,6 +937,7 @@ int decode_variant(DecodeParams& p, const CUtensorMap& map, uint64_t most_cost, 
   const uint32_t fixed = fixed_smem<NT>() + (p.batch + 1) * sizeof(Seq);
   constexpr uint32_t per = STAGE + 8 + 16;
   p.stages = (block_smem<NT>() - fixed) / per;
+  if (p.stages > 32) p.stages = 32;      // a producer lane each
   // a warp's items are at most WARPS + 1 ring positions apart
   static_assert((block_smem<NT>() - fixed_smem<NT>() - (PVLC_KV8_MAX_BATCH + 1) * sizeof(Seq)) / per >=
                     WARPS + 2,
