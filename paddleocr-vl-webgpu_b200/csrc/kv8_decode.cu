@@ -360,58 +360,78 @@ __device__ __forceinline__ void write_out(__half* out, const float (&o)[8], floa
                  pack_half2(o[4] * r, o[5] * r), pack_half2(o[6] * r, o[7] * r));
 }
 
-// The output of a unit from its n blocks' records, in block order: half a warp
-// takes a head, lane `sub` of it dims 8 sub .. + 7 and every 16th record's
-// maximum and sum.  A group of 8 records is read with independent loads.
+// A unit that spans blocks, as this block leaves it for the join.
+struct Split {
+  uint32_t unit;      // b * KV heads + h
+  uint32_t blocks;    // how many it spans (0: no such unit)
+  uint32_t record;    // the first one's record; the others left their first
+};
+
+// The output of head i of a unit from its blocks' records, in block order: 8
+// lanes take a head, lane `sub` dims 16 sub .. + 15 and every 8th record's
+// maximum and sum.  A group of 4 records is read with independent loads, the
+// first one before the maxima are known.
 template <int NT>
-__device__ __forceinline__ void join_blocks(const float* records, uint32_t r0, uint32_t n,
-                                            uint32_t G, __half* out, int warp, int lane) {
-  const uint32_t sub = lane & 15;
+__device__ __forceinline__ void join_head(const float* records, const Split& u, uint32_t i,
+                                          __half* out, uint32_t sub) {
+  constexpr int R = 4;
+  const uint32_t n = u.blocks;
   auto record = [&](uint32_t c) {
-    // record r0 is block c0's second or only one; the others are their blocks' first
-    return records + (size_t)(c == 0 ? r0 : (r0 & ~1u) + 2 * c) * record_floats<NT>();
+    return records + (size_t)(c == 0 ? u.record : (u.record & ~1u) + 2 * c) * record_floats<NT>();
   };
-  for (uint32_t i0 = 2 * warp; i0 < G; i0 += 2 * WARPS) {
-    const uint32_t i = i0 + (lane >> 4);
-    const uint32_t ii = i < G ? i : 0;           // the lanes stay together
-    float m = -CUDART_INF_F;
-    for (uint32_t c = sub; c < n; c += 16) m = fmaxf(m, __ldcg(record(c) + 8 * NT * HD + ii));
+  float4 x[R][4];
+  auto load = [&](uint32_t base) {
 #pragma unroll
-    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (uint32_t base = 0; base < n; base += 8) {
-      float4 x[8][2];
+    for (int e = 0; e < R; ++e)
+      if (base + e < n) {
+        const float4* r = reinterpret_cast<const float4*>(record(base + e) + i * HD + 16 * sub);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (base + e < n) {
-          const float4* r = reinterpret_cast<const float4*>(record(base + e) + ii * HD + 8 * sub);
-          x[e][0] = __ldcg(r);
-          x[e][1] = __ldcg(r + 1);
-        }
-      float f = 0.f, fl = 0.f;
-      if (sub < 8 && base + sub < n) {
-        const float* r = record(base + sub) + 8 * NT * HD + ii;
-        f = fast_exp2(__ldcg(r) - m);
-        fl = __ldcg(r + 8 * NT) * f;
+        for (int d = 0; d < 4; ++d) x[e][d] = __ldcg(r + d);
       }
+  };
+  load(0);
+  float m = -CUDART_INF_F;
+  for (uint32_t c = sub; c < n; c += 8) m = fmaxf(m, __ldcg(record(c) + 8 * NT * HD + i));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float fe = __shfl_sync(0xffffffffu, f, e, 16);
-        l += __shfl_sync(0xffffffffu, fl, e, 16);
-        if (base + e < n) {
-          o[0] += x[e][0].x * fe;
-          o[1] += x[e][0].y * fe;
-          o[2] += x[e][0].z * fe;
-          o[3] += x[e][0].w * fe;
-          o[4] += x[e][1].x * fe;
-          o[5] += x[e][1].y * fe;
-          o[6] += x[e][1].z * fe;
-          o[7] += x[e][1].w * fe;
+  for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float l = 0.f;
+  float4 o[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) o[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+  // the lanes of a warp may have units of different spans: they stay together
+  const uint32_t most = __reduce_max_sync(0xffffffffu, n);
+  for (uint32_t base = 0; base < most; base += R) {
+    float f = 0.f, fl = 0.f;
+    if (sub < R && base + sub < n) {
+      const float* r = record(base + sub) + 8 * NT * HD + i;
+      f = fast_exp2(__ldcg(r) - m);
+      fl = __ldcg(r + 8 * NT) * f;
+    }
+#pragma unroll
+    for (int e = 0; e < R; ++e) {
+      const float fe = __shfl_sync(0xffffffffu, f, e, 8);
+      l += __shfl_sync(0xffffffffu, fl, e, 8);
+      if (base + e < n) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          o[d].x += x[e][d].x * fe;
+          o[d].y += x[e][d].y * fe;
+          o[d].z += x[e][d].z * fe;
+          o[d].w += x[e][d].w * fe;
         }
       }
     }
-    if (i < G) write_out(out + i * HD + 8 * sub, o, l);
+    if (base + R < most) load(base + R);
   }
+  if (n == 0) return;
+  const float r = 1.f / l;
+#pragma unroll
+  for (int d = 0; d < 2; ++d)
+    reinterpret_cast<uint4*>(out + i * HD + 16 * sub)[d] =
+        make_uint4(pack_half2(o[2 * d].x * r, o[2 * d].y * r),
+                   pack_half2(o[2 * d].z * r, o[2 * d].w * r),
+                   pack_half2(o[2 * d + 1].x * r, o[2 * d + 1].y * r),
+                   pack_half2(o[2 * d + 1].z * r, o[2 * d + 1].w * r));
 }
 
 // The units of a block's range [y0, y1): sequence b, KV head h, whose items
@@ -474,6 +494,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   uint64_t* row_full = q_full + 2;                                     // [2]
   uint64_t* slot_empty = row_full + 2;                                 // [2]
   uint32_t* misc = reinterpret_cast<uint32_t*>(q_full + 8);            // [16]
+  Split* splits = reinterpret_cast<Split*>(misc + 8);                  // [2]
   Seq* seq = reinterpret_cast<Seq*>(misc + 16);                        // [B + 1]
   float2* scale = reinterpret_cast<float2*>(seq + B + 1);              // [S]
   uint64_t* full = reinterpret_cast<uint64_t*>(scale + S);             // [S]
@@ -489,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       mbar_init(q_full + i, 32);
       mbar_init(row_full + i, 32);
       mbar_init(slot_empty + i, WARPS);
-      misc[8 + 4 * i] = 0;
+      splits[i].blocks = 0;
     }
     fence_mbar_init();
   }
@@ -695,6 +716,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         }
         __syncwarp();
       }
+      if (lane == 0 && !(it.i0 == 0 && it.has_tail())) {
+        // the unit spans blocks c0 .. c1: it is the last one of c0, the first of the others
+        const uint32_t c0 = owner_of(it.u0, N, C), c1 = owner_of(it.u0 + it.np, N, C);
+        Split& u = splits[it.u0 >= y0 ? 1 : 0];
+        u.unit = it.b * H + it.h;
+        u.blocks = c1 - c0 + 1;
+        u.record = c0 * 2 + (it.u0 >= (uint64_t)c0 * C / N ? 1 : 0);
+      }
       mbar_arrive(row_full + s);
       ++n;
     }
@@ -856,12 +885,6 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           }
         }
       }
-      if (!whole && tid == 0) {         // joined when the block is through
-        uint32_t* e = misc + 8 + (u0 >= y0 ? 4 : 0);
-        e[0] = 1;
-        e[1] = b;
-        e[2] = h;
-      }
       if (it.has_tail() && sq.rows % PAGE == PAGE - 1 && warp < 2) {
         // the open block is full: warp 0 quantises its keys, warp 1 its values
         const int32_t page = p.c.table[(size_t)sq.slot * p.c.max_pages + np];
@@ -883,27 +906,28 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
 
   // -------------------------------------------------- join the blocks
   // At most two units span blocks: one that began in an earlier block (its
-  // record is this block's first) and one that goes on in a later block.
-  __threadfence();
+  // record is this block's first) and one that goes on in a later block.  The
+  // last block to leave a unit's record joins it.
   named_bar_sync(1, CTHREADS);
-  if (tid < 2 && misc[8 + 4 * tid]) {
-    const uint32_t b = misc[9 + 4 * tid], h = misc[10 + 4 * tid];
-    const uint32_t np = seq[b].rows / PAGE;
-    const uint64_t u0 = (uint64_t)seq[b].cost * H + (uint64_t)h * (np + 1 + END_COST);
-    const uint32_t c0 = owner_of(u0, N, C), c1 = owner_of(u0 + np, N, C);
-    uint32_t* ticket = p.tickets + b * H + h;
-    const bool mine = atomicAdd(ticket, 1) == c1 - c0;
-    if (mine) *ticket = 0;
-    misc[8 + 4 * tid] = mine ? c1 - c0 + 1 : 0;
-    misc[11 + 4 * tid] = c0 * 2 + (u0 >= (uint64_t)c0 * C / N ? 1 : 0);   // block c0's record
+  if (tid < 2 && splits[tid].blocks) {
+    __threadfence();
+    uint32_t* ticket = p.tickets + splits[tid].unit;
+    const bool mine = atomicAdd(ticket, 1) == splits[tid].blocks - 1;
+    if (mine) {
+      *ticket = 0;
+      __threadfence();
+    } else {
+      splits[tid].blocks = 0;
+    }
   }
   named_bar_sync(1, CTHREADS);
-  for (int s = 0; s < 2; ++s) {
-    const uint32_t n = misc[8 + 4 * s];
-    if (n == 0) continue;
-    __threadfence();
-    join_blocks<NT>(p.records, misc[11 + 4 * s], n, G,
-                    p.out + ((size_t)misc[9 + 4 * s] * H + misc[10 + 4 * s]) * G * HD, warp, lane);
+  if (splits[0].blocks + splits[1].blocks == 0) return;
+  // 8 lanes take a (unit, head)
+  for (uint32_t k = tid >> 3; k < 2 * 8 * NT; k += CTHREADS / 8) {
+    Split u = splits[k & 1];
+    const uint32_t i = k >> 1;
+    if (i >= G) u.blocks = 0;
+    join_head<NT>(p.records, u, i, p.out + (size_t)u.unit * G * HD, lane & 7);
   }
 }
 
