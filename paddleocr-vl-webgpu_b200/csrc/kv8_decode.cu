@@ -54,7 +54,7 @@ constexpr int WARPS = KV8_WARPS;                  // consumer warps
 constexpr int THREADS = (WARPS + 2) * 32;         // + the producer and the sequence warp
 constexpr int CTHREADS = WARPS * 32;
 constexpr uint32_t STAGE = 8192;                  // a page's K and V codes of one head
-constexpr uint32_t END_COST = 3;                  // a unit's end, in pages
+constexpr uint32_t END_COST = 8;                  // a unit's end, in pages
 constexpr uint32_t MIN_COST = 8;                  // least work of a block, in pages
 constexpr int ACC_PITCH = HD + 4;
 constexpr float W_SHIFT = 14.f;
@@ -333,6 +333,12 @@ __device__ __forceinline__ uint32_t owner_of(uint64_t y, uint64_t G, uint64_t C)
   return static_cast<uint32_t>(((y + 1) * G + C - 1) / C - 1);
 }
 
+// floor(i C / N): where block i's range begins.
+__device__ __forceinline__ uint64_t cut_at(uint64_t i, uint64_t C, uint64_t N) {
+  const uint64_t x = i * C;
+  return x >> 32 ? x / N : (uint32_t)x / (uint32_t)N;
+}
+
 struct Seq {
   uint32_t cost;     // cost position of the sequence's first unit, per KV head
   int32_t slot, rows;
@@ -435,7 +441,8 @@ __device__ __forceinline__ void join_head(const float* records, const Split& u, 
 }
 
 // The units of a block's range [y0, y1): sequence b, KV head h, whose items
-// [i0, i1) of np pages and a tail (item np) are the block's.
+// [i0, i1) are the block's: item 0 is the tail, item i > 0 page i - 1.  The tail
+// comes first so that its latency passes under the pages' stream.
 struct Units {
   const Seq* seq;
   uint32_t B, H, b, h, np, i0, i1;
@@ -445,7 +452,8 @@ struct Units {
                                    uint64_t y1_, uint32_t b_)
       : seq(seq_), B(B_), H(H_), b(b_), y0(y0_), y1(y1_) {
     const uint32_t len = seq[b].rows / PAGE + 1 + END_COST;
-    h = (uint32_t)((y0 - (uint64_t)seq[b].cost * H) / len);
+    const uint64_t past = y0 - (uint64_t)seq[b].cost * H;     // below H len
+    h = past >> 32 ? (uint32_t)(past / len) : (uint32_t)past / len;
     set();
   }
   __device__ __forceinline__ void set() {
@@ -457,8 +465,13 @@ struct Units {
     i1 = u0 < y1 ? min((uint32_t)umin64(y1 - u0, len), np + 1) : 0;
   }
   __device__ __forceinline__ bool valid() const { return b < B && u0 < y1; }
-  __device__ __forceinline__ bool has_pages() const { return i0 < i1; }
-  __device__ __forceinline__ bool has_tail() const { return i1 == np + 1; }
+  __device__ __forceinline__ bool has_items() const { return i0 < i1; }
+  __device__ __forceinline__ bool has_tail() const { return i0 == 0; }
+  __device__ __forceinline__ bool whole() const { return i0 == 0 && i1 == np + 1; }
+  // ring positions: a tail takes two, K and V
+  __device__ __forceinline__ uint32_t positions() const {
+    return has_items() ? i1 - i0 + (has_tail() ? 1 : 0) : 0;
+  }
   __device__ __forceinline__ void step() {
     if (++h == H) {
       h = 0;
@@ -557,9 +570,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   }
   const uint64_t C = (uint64_t)seq[B].cost * H;
   if (C == 0) return;
-  const uint64_t N = umax64(1, umin64(gridDim.x, C / MIN_COST));
+  const uint64_t N = C / MIN_COST >= gridDim.x ? gridDim.x : umax64(1, C / MIN_COST);
   if (blockIdx.x >= N) return;
-  const uint64_t y0 = blockIdx.x * C / N, y1 = (blockIdx.x + 1) * C / N;
+  const uint64_t y0 = cut_at(blockIdx.x, C, N), y1 = cut_at(blockIdx.x + 1, C, N);
   // the last sequence whose line starts at or before y (idle ones have no length)
   auto seq_at = [&](uint64_t y) -> uint32_t {
     uint32_t lo = 0, hi = B;
@@ -581,12 +594,13 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     int32_t page = -1;                // >= 0: a page; -1: an id out of range; -2, -3: K, V tail
     auto find = [&](uint32_t k) {     // the item of ring position k; false behind the last
       while (it.valid()) {
-        const uint32_t n = it.has_pages() ? it.i1 - it.i0 + (it.has_tail() ? 1 : 0) : 0;
+        const uint32_t n = it.positions();
         if (k < base + n) {
-          const uint32_t i = it.i0 + (k - base);
-          if (i >= it.np) {
-            page = -2 - (int32_t)(i - it.np);
+          const uint32_t j = k - base;
+          if (it.has_tail() && j < 2) {
+            page = -2 - (int32_t)j;
           } else {
+            const uint32_t i = it.has_tail() ? j - 2 : it.i0 - 1 + j;
             page = p.c.table[(size_t)it.sq.slot * p.c.max_pages + i];
             if (page < 0 || (uint32_t)page >= p.c.pages) page = -1;
           }
@@ -668,7 +682,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
     Units it(seq, B, H, y0, y1, seq_at(y0));
     uint32_t n = 0;
     for (; it.valid(); it.step()) {
-      if (!it.has_pages()) continue;
+      if (!it.has_items()) continue;
       const uint32_t s = n & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(slot_empty + s, (n >> 1 & 1) ^ 1))) {
         if (lane == 0) atomicOr(p.flags, kFlagTimeout);
@@ -716,15 +730,33 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         }
         __syncwarp();
       }
-      if (lane == 0 && !(it.i0 == 0 && it.has_tail())) {
+      if (lane == 0 && !it.whole()) {
         // the unit spans blocks c0 .. c1: it is the last one of c0, the first of the others
         const uint32_t c0 = owner_of(it.u0, N, C), c1 = owner_of(it.u0 + it.np, N, C);
         Split& u = splits[it.u0 >= y0 ? 1 : 0];
         u.unit = it.b * H + it.h;
         u.blocks = c1 - c0 + 1;
-        u.record = c0 * 2 + (it.u0 >= (uint64_t)c0 * C / N ? 1 : 0);
+        u.record = c0 * 2 + (it.u0 >= cut_at(c0, C, N) ? 1 : 0);
       }
       mbar_arrive(row_full + s);
+      if (it.has_tail() && it.sq.rows % PAGE == PAGE - 1) {
+        // the open block is full: its rows (the last one just written by this warp) to its page
+        const int32_t page = p.c.table[(size_t)it.sq.slot * p.c.max_pages + it.np];
+        if (page < 0 || (uint32_t)page >= p.c.pages) {
+          if (lane == 0) atomicOr(p.flags, kFlagPage);
+        } else {
+#pragma unroll 1
+          for (uint32_t kv = 0; kv < 2; ++kv) {
+            const uint4* from = reinterpret_cast<const uint4*>(tail_rows(p.c, it.sq.slot, kv, it.h));
+            uint4 x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              x[e] = from[(e >> 1) * 64 + (lane >> 3) * 16 + (lane & 7) * 2 + (e & 1)];
+            quantise_block<CODE>(x, block_codes(p.c, page, kv, it.h),
+                                 p.c.scales + ((size_t)page * H + it.h) * 2 + kv, lane);
+          }
+        }
+      }
       ++n;
     }
     return;
@@ -771,9 +803,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   uint32_t unit = 0;                  // units of this block so far
   for (Units it(seq, B, H, y0, y1, seq_at(y0)); it.valid(); it.step()) {
     const Seq sq = it.sq;
-    const uint32_t b = it.b, h = it.h, np = it.np, i0 = it.i0, i1 = it.i1;
+    const uint32_t b = it.b, h = it.h, i0 = it.i0, i1 = it.i1;
     const uint64_t u0 = it.u0;
-    if (it.has_pages()) {
+    if (it.has_items()) {
       // ---------------------------------------------- this block's pages
       Acc<NT> a;
 #pragma unroll
@@ -800,23 +832,16 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
             qf[nt][4 * e + 2] = x.z;
             qf[nt][4 * e + 3] = x.w;
           }
-        for (uint32_t i = i0 + first; i < i1; i += WARPS) {
-          seek(at + i - i0);
-          if (i < np) {
-            if (landed()) {
-              const float2 sc = scale[stage];
-              page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, a, g, t);
-            }
-            release(stage);
-            continue;
-          }
-          // ----------------------------------------------------------- tail
+        uint32_t i = i0 + first;
+        if (i == 0) {
+          // --------------------------------------------------------- tail
+          seek(at);
           const int last = sq.rows % PAGE;
           const uint8_t* rows = slot + NT * 2048;
           const uint32_t s0 = stage;
           landed();
           const uint8_t* kt = ring + stage * STAGE;
-          seek(at + i - i0 + 1);
+          seek(at + 1);
           landed();
           const uint8_t* vt = ring + stage * STAGE;
           if (arrived(row_full + (unit & 1), slot_phase)) {
@@ -824,6 +849,16 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           }
           release(stage);
           release(s0);
+          i += WARPS;
+        }
+        const uint32_t skew = it.has_tail() ? 1 : 0;
+        for (; i < i1; i += WARPS) {
+          seek(at + i - i0 + skew);
+          if (landed()) {
+            const float2 sc = scale[stage];
+            page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, a, g, t);
+          }
+          release(stage);
         }
       }
       // the row barrier advances with the slot, also past warps that do not use it
@@ -831,7 +866,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       __syncwarp();
       if (alive && lane == 0) mbar_arrive(slot_empty + (unit & 1));
       ++unit;
-      at += i1 - i0 + (i1 == np + 1 ? 1 : 0);
+      at += it.positions();
       turn = (turn + i1 - i0) % WARPS;
       // ------------------------------------------------- join the warps
 #pragma unroll
@@ -856,7 +891,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       }
       named_bar_sync(1, CTHREADS);
       // half a warp takes a head, each lane 8 of its dims
-      const bool whole = i0 == 0 && i1 == np + 1;
+      const bool whole = it.whole();
       float* rec = p.records + (size_t)(blockIdx.x * 2 + (u0 >= y0 ? 1 : 0)) * record_floats<NT>();
       __half* out = p.out + ((size_t)b * H + h) * G * HD;
       const uint32_t sub = lane & 15;
@@ -883,21 +918,6 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
             rec[8 * NT * HD + i] = m;
             rec[8 * NT * (HD + 1) + i] = l;
           }
-        }
-      }
-      if (it.has_tail() && sq.rows % PAGE == PAGE - 1 && warp < 2) {
-        // the open block is full: warp 0 quantises its keys, warp 1 its values
-        const int32_t page = p.c.table[(size_t)sq.slot * p.c.max_pages + np];
-        if (page < 0 || (uint32_t)page >= p.c.pages) {
-          if (lane == 0) atomicOr(p.flags, kFlagPage);
-        } else {
-          const uint4* from = reinterpret_cast<const uint4*>(tail_rows(p.c, sq.slot, warp, h));
-          uint4 x[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            x[e] = from[(e >> 1) * 64 + (lane >> 3) * 16 + (lane & 7) * 2 + (e & 1)];
-          quantise_block<CODE>(x, block_codes(p.c, page, warp, h),
-                               p.c.scales + ((size_t)page * H + h) * 2 + warp, lane);
         }
       }
       named_bar_sync(1, CTHREADS);     // the unit's buffers have been read
