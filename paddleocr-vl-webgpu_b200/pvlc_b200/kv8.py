@@ -28,41 +28,54 @@ FLAG_ROWS_HELD, FLAG_ROPE_ROW, FLAG_TIMEOUT = 1, 2, 8
 FLAG_PAGE, FLAG_SLOT, FLAG_EXHAUSTED, FLAG_INPUT_ROWS = 16, 32, 64, 128
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+# The current device and a stream's handle as plain numbers: the checks below run once for
+# every layer of every decode step, so they ask torch for as little as they can.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _need(t, dtype, shape, device, name):
+def _need(t, dtype, shape, index, name):
+    """A contiguous tensor of this type and shape on CUDA device `index`."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index
+            and t.shape == shape and t.is_contiguous()):
+        return
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the cache on cuda:{index}")
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
 
 
-def _rows(t, heads, device, name):
-    """A [rows, heads, 128] fp16 tensor whose rows may sit apart; the stride in elements."""
+def _rows(t, heads, index, name):
+    """A [rows, heads, 128] fp16 tensor whose rows may sit apart; (rows, stride in elements)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype is not torch.float16:
         raise TypeError(f"{name} must be torch.float16, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != HD:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected (rows, {heads}, {HD})")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the cache on cuda:{index}")
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != HD:
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected (rows, {heads}, {HD})")
     s0, s1, s2 = t.stride()
     if s2 != 1 or (heads > 1 and s1 != HD):
         raise ValueError(f"{name}: each row must be contiguous")
-    if t.shape[0] == 1:
-        return heads * HD
+    if shape[0] == 1:
+        return 1, heads * HD
     if s0 >= 1 << 32:
         raise ValueError(f"{name}: rows are too far apart")
-    return s0
+    return shape[0], s0
+
+
+def _batch(slot):
+    """The number of sequences a slot tensor names."""
+    if not isinstance(slot, torch.Tensor):
+        raise TypeError("slot must be a CUDA tensor")
+    return slot.numel()
 
 
 class Cache:
@@ -85,13 +98,13 @@ class Cache:
             raise ValueError("table must be [slots, max_pages]")
         L, P, _, H = codes.shape[:4]
         S, M = table.shape
-        self.device = dev = codes.device
-        _need(codes, codes.dtype, codes.shape, dev, "codes")
-        _need(scales, torch.float32, (L, P, H, 2), dev, "scales")
-        _need(tails, torch.float16, (L, S, 2, H, PAGE, HD), dev, "tails")
-        _need(table, torch.int32, (S, M), dev, "table")
-        _need(tokens, torch.int32, (S,), dev, "tokens")
-        _need(refs, torch.int32, (P,), dev, "refs")
+        self.device, self.index = codes.device, codes.get_device()
+        _need(codes, codes.dtype, codes.shape, self.index, "codes")
+        _need(scales, torch.float32, (L, P, H, 2), self.index, "scales")
+        _need(tails, torch.float16, (L, S, 2, H, PAGE, HD), self.index, "tails")
+        _need(table, torch.int32, (S, M), self.index, "table")
+        _need(tokens, torch.int32, (S,), self.index, "tokens")
+        _need(refs, torch.int32, (P,), self.index, "refs")
         self.codes, self.scales, self.tails = codes, scales, tails
         self.table, self.tokens, self.refs = table, tokens, refs
         self.layers, self.pages, self.slots, self.max_pages, self.kv_heads = L, P, S, M, H
@@ -129,7 +142,7 @@ class Workspace:
     batches up to `batch` sequences of `query_heads` heads.  One stream at a time."""
 
     def __init__(self, cache: Cache, batch: int, query_heads: int | None = None):
-        self.device = cache.device
+        self.device, self.index = cache.device, cache.index
         self.nbytes = int(abi.lib().pvlc_attn_kv8_workspace_bytes(
             int(batch), int(query_heads or cache.kv_heads), cache.kv_heads, cache.slots,
             cache.pages))
@@ -138,26 +151,29 @@ class Workspace:
         self.buffer = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device)
         self._p = self.buffer.data_ptr()
         with torch.cuda.device(self.device):
-            abi.check(abi.lib().pvlc_attn_kv8_workspace_init(self._p, self.nbytes, _stream()),
-                      "pvlc_attn_kv8_workspace_init")
+            abi.check(abi.lib().pvlc_attn_kv8_workspace_init(
+                self._p, self.nbytes, _raw_stream(self.index)), "pvlc_attn_kv8_workspace_init")
 
     def errors(self) -> int:
         """Read and clear the fault word (FLAG_* bits); waits for the current stream."""
         flags = ctypes.c_uint32(0)
-        st = abi.lib().pvlc_attn_kv8_errors(self._p, ctypes.byref(flags), _stream())
+        st = abi.lib().pvlc_attn_kv8_errors(self._p, ctypes.byref(flags),
+                                            _raw_stream(self.index))
         if st not in (abi.OK, abi.DEVICE_FAULT_FLAG):
             abi.check(st, "pvlc_attn_kv8_errors")
         return int(flags.value)
 
 
-def _call(cache, workspace, *others):
-    """The checks that every call shares: one device, and that the current one."""
+def _call(cache, workspace):
+    """What every call checks: a cache and a workspace on the current device.  Returns it."""
     if not isinstance(cache, Cache) or not isinstance(workspace, Workspace):
         raise TypeError("expected a kv8.Cache and a kv8.Workspace")
-    if workspace.device != cache.device:
+    index = cache.index
+    if workspace.index != index:
         raise ValueError(f"the workspace is on {workspace.device}, the cache on {cache.device}")
-    if cache.device.index != torch.cuda.current_device():
+    if index != _current_device():
         raise ValueError(f"the cache is on {cache.device}, which is not the current device")
+    return index
 
 
 def store(cache: Cache, layer: int, k, v, begin, count, slot, max_count: int,
@@ -167,22 +183,22 @@ def store(cache: Cache, layer: int, k, v, begin, count, slot, max_count: int,
     k, v: [rows, kv_heads, 128] fp16, keys rotated, rows the same distance apart in both;
     sequence b takes rows begin[b] : begin[b] + count[b] (int32 device tensors, count <=
     max_count) behind the rows its slot holds."""
-    _call(cache, workspace)
-    dev = cache.device
-    ks, vs = _rows(k, cache.kv_heads, dev, "k"), _rows(v, cache.kv_heads, dev, "v")
-    if ks != vs or k.shape[0] != v.shape[0]:
+    index = _call(cache, workspace)
+    n, stride = _rows(k, cache.kv_heads, index, "k")
+    if _rows(v, cache.kv_heads, index, "v") != (n, stride):
         raise ValueError("k and v must have the same rows, the same distance apart")
-    B = slot.shape[0]
-    _need(slot, torch.int32, (B,), dev, "slot")
-    _need(begin, torch.int32, (B,), dev, "begin")
-    _need(count, torch.int32, (B,), dev, "count")
+    B = _batch(slot)
+    _need(slot, torch.int32, (B,), index, "slot")
+    _need(begin, torch.int32, (B,), index, "begin")
+    _need(count, torch.int32, (B,), index, "count")
     if not 0 <= layer < cache.layers or max_count < 0:
         raise ValueError("layer or max_count out of range")
     st = abi.lib().pvlc_attn_kv8_store(
-        cache._p, layer, k.data_ptr(), v.data_ptr(), k.shape[0], ks, begin.data_ptr(),
+        cache._p, layer, k.data_ptr(), v.data_ptr(), n, stride, begin.data_ptr(),
         count.data_ptr(), slot.data_ptr(), B, max_count, workspace._p, workspace.nbytes,
-        _stream())
-    abi.check(st, "pvlc_attn_kv8_store")
+        _raw_stream(index))
+    if st:
+        abi.check(st, "pvlc_attn_kv8_store")
 
 
 def decode(cache: Cache, layer: int, q, k_new, v_new, rope_cos, rope_sin, slot,
@@ -194,41 +210,44 @@ def decode(cache: Cache, layer: int, q, k_new, v_new, rope_cos, rope_sin, slot,
     row-strided view (column blocks of one projection; k_new and v_new alike); rope tables
     [3, R, 128] f32; rope_row int32 [B] (None: the rows the slot holds); slot int32 [B] (None:
     sequence b is slot b).  Returns [B, query_heads, 128] fp16."""
-    _call(cache, workspace)
-    dev, H = cache.device, cache.kv_heads
-    B, QH = q.shape[0], q.shape[1]
-    qs = _rows(q, QH, dev, "q")
-    ks, vs = _rows(k_new, H, dev, "k_new"), _rows(v_new, H, dev, "v_new")
-    if ks != vs or k_new.shape[0] != B or v_new.shape[0] != B:
+    index, H = _call(cache, workspace), cache.kv_heads
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise TypeError("q must be a [B, query_heads, 128] CUDA tensor")
+    if not isinstance(rope_cos, torch.Tensor) or rope_cos.dim() != 3:
+        raise TypeError("rope_cos must be a [3, R, 128] CUDA tensor")
+    QH, R = q.shape[1], rope_cos.shape[1]
+    B, qs = _rows(q, QH, index, "q")
+    kb, ks = _rows(k_new, H, index, "k_new")
+    if kb != B or _rows(v_new, H, index, "v_new") != (B, ks):
         raise ValueError("k_new and v_new must have q's rows, the same distance apart")
-    R = rope_cos.shape[1]
-    _need(rope_cos, torch.float32, (3, R, HD), dev, "rope_cos")
-    _need(rope_sin, torch.float32, (3, R, HD), dev, "rope_sin")
+    _need(rope_cos, torch.float32, (3, R, HD), index, "rope_cos")
+    _need(rope_sin, torch.float32, (3, R, HD), index, "rope_sin")
     sp = rp = None
     if slot is not None:
-        _need(slot, torch.int32, (B,), dev, "slot")
+        _need(slot, torch.int32, (B,), index, "slot")
         sp = slot.data_ptr()
     if rope_row is not None:
-        _need(rope_row, torch.int32, (B,), dev, "rope_row")
+        _need(rope_row, torch.int32, (B,), index, "rope_row")
         rp = rope_row.data_ptr()
     if out is None:
-        out = torch.empty((B, QH, HD), dtype=torch.float16, device=dev)
+        out = q.new_empty((B, QH, HD))
     else:
-        _need(out, torch.float16, (B, QH, HD), dev, "out")
+        _need(out, torch.float16, (B, QH, HD), index, "out")
     if not 0 <= layer < cache.layers:
         raise ValueError("layer out of range")
     st = abi.lib().pvlc_attn_kv8_decode(
         cache._p, layer, q.data_ptr(), qs, k_new.data_ptr(), v_new.data_ptr(), ks, QH,
         rope_cos.data_ptr(), rope_sin.data_ptr(), R, rp, sp, B, workspace._p, workspace.nbytes,
-        out.data_ptr(), _stream())
-    abi.check(st, "pvlc_attn_kv8_decode")
+        out.data_ptr(), _raw_stream(index))
+    if st:
+        abi.check(st, "pvlc_attn_kv8_decode")
     return out
 
 
-def _amount(x, B, dev, name):
+def _amount(x, B, index, name):
     """(device pointer, 0) of a per-sequence tensor, or (None, rows) of one number."""
     if isinstance(x, torch.Tensor):
-        _need(x, torch.int32, (B,), dev, name)
+        _need(x, torch.int32, (B,), index, name)
         return x.data_ptr(), 0
     if not 0 <= x < 1 << 31:
         raise ValueError(f"{name} out of range")
@@ -238,32 +257,33 @@ def _amount(x, B, dev, name):
 def grow(cache: Cache, slot, workspace: Workspace, advance=0, ahead=0):
     """Advance sequences by `advance` rows and give them the pages of their next `ahead` rows
     (each a number, or an int32 tensor per sequence; pvlc_attn_kv8_grow)."""
-    _call(cache, workspace)
-    B = slot.shape[0]
-    _need(slot, torch.int32, (B,), cache.device, "slot")
-    ap, an = _amount(advance, B, cache.device, "advance")
-    hp, hn = _amount(ahead, B, cache.device, "ahead")
+    index, B = _call(cache, workspace), _batch(slot)
+    _need(slot, torch.int32, (B,), index, "slot")
+    ap, an = _amount(advance, B, index, "advance")
+    hp, hn = _amount(ahead, B, index, "ahead")
     st = abi.lib().pvlc_attn_kv8_grow(cache._p, slot.data_ptr(), B, ap, an, hp, hn, workspace._p,
-                                      workspace.nbytes, _stream())
-    abi.check(st, "pvlc_attn_kv8_grow")
+                                      workspace.nbytes, _raw_stream(index))
+    if st:
+        abi.check(st, "pvlc_attn_kv8_grow")
 
 
 def fork(cache: Cache, slot, parent, workspace: Workspace, advance: int = 0, out=None):
     """Sequence b becomes a copy of sequence parent[b] (int32 [B], -1: none), after every
     sequence has grown by `advance` rows; returns the new slots (pvlc_attn_kv8_fork)."""
-    _call(cache, workspace)
-    dev, B = cache.device, slot.shape[0]
-    _need(slot, torch.int32, (B,), dev, "slot")
-    _need(parent, torch.int32, (B,), dev, "parent")
+    index, B = _call(cache, workspace), _batch(slot)
+    _need(slot, torch.int32, (B,), index, "slot")
+    _need(parent, torch.int32, (B,), index, "parent")
     if out is None:
         out = torch.empty_like(slot)
     else:
-        _need(out, torch.int32, (B,), dev, "out")
+        _need(out, torch.int32, (B,), index, "out")
     if not 0 <= advance < 1 << 31:
         raise ValueError("advance out of range")
     st = abi.lib().pvlc_attn_kv8_fork(cache._p, slot.data_ptr(), parent.data_ptr(), B, advance,
-                                      out.data_ptr(), workspace._p, workspace.nbytes, _stream())
-    abi.check(st, "pvlc_attn_kv8_fork")
+                                      out.data_ptr(), workspace._p, workspace.nbytes,
+                                      _raw_stream(index))
+    if st:
+        abi.check(st, "pvlc_attn_kv8_fork")
     return out
 
 
@@ -271,14 +291,15 @@ def compact(cache: Cache, into: Cache, workspace: Workspace, live=None):
     """Copy the live pages, in order, to the front of another cache with the same layers,
     heads and type, and make its tables match (pvlc_attn_kv8_compact).  live: optional int32
     [1] tensor that receives the number of live pages (-1: they do not fit)."""
-    _call(cache, workspace)
+    index = _call(cache, workspace)
     if not isinstance(into, Cache):
         raise TypeError("into must be a kv8.Cache")
-    if into.device != cache.device:
+    if into.index != index:
         raise ValueError(f"into is on {into.device}, the cache on {cache.device}")
     if live is not None:
-        _need(live, torch.int32, (1,), cache.device, "live")
+        _need(live, torch.int32, (1,), index, "live")
     st = abi.lib().pvlc_attn_kv8_compact(cache._p, into._p,
                                          live.data_ptr() if live is not None else None,
-                                         workspace._p, workspace.nbytes, _stream())
-    abi.check(st, "pvlc_attn_kv8_compact")
+                                         workspace._p, workspace.nbytes, _raw_stream(index))
+    if st:
+        abi.check(st, "pvlc_attn_kv8_compact")

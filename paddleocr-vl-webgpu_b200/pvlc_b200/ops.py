@@ -440,32 +440,35 @@ def beam_topk(logits, scores, topk: int, workspace: BeamWorkspace | None = None,
         raise TypeError("logits must be a CUDA tensor")
     if logits.dtype not in (torch.float32, torch.float16):
         raise TypeError(f"logits must be float32 or float16, got {logits.dtype}")
-    dev = logits.device
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"logits are on {dev}, which is not the current device")
-    if scores.dim() != 2 or logits.dim() != 2:
-        raise ValueError("logits must be [B * W, vocab] and scores [B, W]")
-    B, W = scores.shape
-    rows, V = logits.shape
-    _need(scores, torch.float32, (B, W), "scores")
-    if rows != B * W or logits.stride(1) != 1:
+    index = logits.get_device()
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"logits are on {logits.device}, which is not the current device")
+    if not isinstance(scores, torch.Tensor) or scores.dim() != 2 or logits.dim() != 2:
+        raise TypeError("logits must be [B * W, vocab] and scores [B, W] CUDA tensors")
+    (B, W), (rows, V) = scores.shape, logits.shape
+    stride, unit = logits.stride()
+    _need(scores, torch.float32, None, "scores")
+    if rows != B * W or unit != 1:
         raise ValueError(f"logits must be {B * W} rows of contiguous values")
     if out is None:
-        out = (torch.empty((B, topk), dtype=torch.float32, device=dev),
-               torch.empty((B, topk), dtype=torch.int32, device=dev),
-               torch.empty((B, topk), dtype=torch.int32, device=dev))
+        # one allocation for the three
+        score, beam, token = torch.empty((3, B, topk), dtype=torch.int32,
+                                         device=logits.device).unbind(0)
+        out = (score.view(torch.float32), beam, token)
     else:
         for t, dt, name in zip(out, (torch.float32, torch.int32, torch.int32),
                                ("score", "beam", "token")):
             _need(t, dt, (B, topk), name)
     if workspace is None:
-        workspace = BeamWorkspace(B, W, V, topk, dev)
-    if any(t.device != dev for t in (scores, workspace.buffer) + tuple(out)):
+        workspace = BeamWorkspace(B, W, V, topk, logits.device)
+    if not (scores.get_device() == workspace.buffer.get_device() == out[0].get_device() ==
+            out[1].get_device() == out[2].get_device() == index):
         raise ValueError("logits, scores, workspace and out must be on one device")
     st = abi.lib().pvlc_lm_head_beam_topk(
-        logits.data_ptr(), int(logits.dtype == torch.float16),
-        logits.stride(0) if rows > 1 else max(V, logits.stride(0)), scores.data_ptr(), B, W, V,
-        topk, workspace.buffer.data_ptr(), workspace.nbytes, out[0].data_ptr(),
-        out[1].data_ptr(), out[2].data_ptr(), torch.cuda.current_stream().cuda_stream)
-    abi.check(st, "pvlc_lm_head_beam_topk")
-    return tuple(out)
+        logits.data_ptr(), int(logits.dtype is torch.float16),
+        stride if rows > 1 else max(V, stride), scores.data_ptr(), B, W, V, topk,
+        workspace.buffer.data_ptr(), workspace.nbytes, out[0].data_ptr(), out[1].data_ptr(),
+        out[2].data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        abi.check(st, "pvlc_lm_head_beam_topk")
+    return out
