@@ -8,24 +8,33 @@
 // the lower token.  Within a beam the order is that of the logits, so each
 // row's K best logits are enough, and they need no logarithm.
 //
-// One pass over the logits: a block holds a chunk of a row in registers, sums
-// its exponentials against its own maximum and keeps its K best logits as
-// 64-bit keys (ordered logit, then ~token).  A block per request then joins
-// the chunks: the rows' log-sums in f64, so that candidates of two beams that
-// differ by more than 1e-7 are told apart, and the K best of all.
+// One pass over the logits, bound by HBM: a block holds a chunk of a row in
+// registers, sums its exponentials against its own maximum and keeps its K best
+// logits as 64-bit keys (ordered logit, then ~token), best first.  A block per
+// request then joins the chunks: the rows' log-sums in f64, so that candidates
+// of two beams that differ by more than 1e-7 are told apart, and the K best.
+//
+// Selection: the K-th best of any disjoint groups' best elements is a bound that
+// at least K elements reach, so only what reaches it is looked at -- in a chunk,
+// the K-th best of a warp's 32 lane maxima; in a join, the K-th best of the
+// chunks' best -- a few dozen elements, which are ranked by counting.  Where too
+// many reach the bound (equal or masked logits) the K are taken one at a time.
+// Keys are unique, so nothing depends on the order in which threads arrive.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
+#include <string.h>
 
+#include "pvlc_common.cuh"
 #include "pvlc_internal.h"
 
 namespace pvlc {
 namespace beam {
 
 constexpr int THREADS = 256;
-constexpr int PER = 32;                      // logits a thread
-constexpr uint32_t CHUNK = THREADS * PER;
+constexpr uint32_t LIST = 512;               // elements ranked by counting
+constexpr uint32_t MAX_HEADS = 512;          // chunks of a request that a join bounds by
 
 typedef unsigned long long u64;
 
@@ -80,38 +89,108 @@ struct Params {
   int32_t* out_token;
 };
 
-template <typename T>
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+// PER logits a thread; VEC: rows are 16-byte aligned and read so.
+template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(THREADS) beam_chunk_kernel(const Params p) {
-  const uint32_t row = blockIdx.y, c = blockIdx.x;
+  constexpr uint32_t CHUNK = THREADS * PER;
+  constexpr int W = VEC ? 16 / sizeof(T) : 1;        // logits of one load
+  __shared__ float warp_top[THREADS / 32], warp_bound[THREADS / 32];
+  __shared__ u64 list[LIST];
+  __shared__ uint32_t listed;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t row = blockIdx.y, c = blockIdx.x, K = p.topk;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+  // token of v[i]: loads of W neighbours, THREADS loads apart
+  auto token = [&](int i) { return c * CHUNK + (i / W * THREADS + threadIdx.x) * W + i % W; };
   float v[PER];
-  u64 best = 0;       // below every logit's key
+  if (VEC && (c + 1) * CHUNK <= p.vocab) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const uint32_t at = c * CHUNK + i * THREADS + threadIdx.x;
-    v[i] = at < p.vocab ? (float)x[at] : -CUDART_INF_F;
-    const u64 key = at < p.vocab ? (u64)ordered(v[i]) << 32 | (0xffffffffu - at) : 0;
-    best = key > best ? key : best;
-  }
-  u64 top = block_max(best);
-  const float m = from_ordered((uint32_t)(top >> 32));
-  float s = 0.f;
+    for (int i = 0; i < PER; i += W) {
+      const uint4 y = __ldg(reinterpret_cast<const uint4*>(x + token(i)));
+      T z[W];
+      memcpy(z, &y, sizeof(T) * W);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) s += v[i] > -CUDART_INF_F ? expf(v[i] - m) : 0.f;
-  s = block_sum(s);
-  const size_t slot = (size_t)row * p.chunks + c;
-  if (threadIdx.x == 0) p.sums[slot] = make_float2(m, s);
-  for (uint32_t k = 0; k < p.topk; ++k) {
-    if (threadIdx.x == 0) p.keys[slot * p.topk + k] = top;
-    if (top == 0) continue;                  // fewer logits than K
-    best = 0;
+      for (int e = 0; e < W; ++e) v[i + e] = to_float(z[e]);
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const uint32_t at = c * CHUNK + i * THREADS + threadIdx.x;
-      const u64 key = at < p.vocab ? (u64)ordered(v[i]) << 32 | (0xffffffffu - at) : 0;
-      if (key < top && key > best) best = key;
+      const uint32_t at = token(i);
+      v[i] = at < p.vocab ? to_float(x[at]) : -CUDART_INF_F;
     }
-    top = block_max(best);
+  }
+  float best = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) best = fmaxf(best, v[i]);    // a NaN counts as -infinity
+  // lane maxima in descending order: the K-th is the warp's bound
+  float sorted = best;
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j; j >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, sorted, j);
+      const bool up = ((lane & k) == 0) == ((lane & j) == 0);
+      sorted = up ? fmaxf(sorted, y) : fminf(sorted, y);
+    }
+  const float kth = __shfl_sync(0xffffffffu, sorted, K <= 32 ? K - 1 : 31);
+  if (lane == 0) {
+    warp_top[warp] = sorted;
+    warp_bound[warp] = kth;
+  }
+  if (threadIdx.x == 0) listed = 0;
+  __syncthreads();
+  float m = warp_top[0], bound = warp_bound[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 32; ++w) {
+    m = fmaxf(m, warp_top[w]);
+    bound = fmaxf(bound, warp_bound[w]);
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    s += v[i] > -CUDART_INF_F ? exp2f((v[i] - m) * 1.4426950408889634f) : 0.f;
+  const size_t slot = (size_t)row * p.chunks + c;
+  u64* keys = p.keys + slot * K;
+  auto key_of = [&](int i) -> u64 {
+    return token(i) < p.vocab ? (u64)ordered(v[i]) << 32 | (0xffffffffu - token(i)) : 0;
+  };
+  if (K <= 32 && bound > -CUDART_INF_F) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (v[i] >= bound) {
+        const uint32_t at = atomicAdd(&listed, 1);
+        if (at < LIST) list[at] = key_of(i);
+      }
+  } else if (threadIdx.x == 0) {
+    listed = LIST + 1;
+  }
+  s = block_sum(s);                        // its barriers also publish the list
+  if (threadIdx.x == 0) p.sums[slot] = make_float2(m, s);
+  const uint32_t n = listed;
+  if (n <= LIST) {
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+      const u64 mine = list[i];
+      uint32_t rank = 0;
+      for (uint32_t j = 0; j < n; ++j) rank += list[j] > mine;
+      if (rank < K) keys[rank] = mine;
+    }
+    return;
+  }
+  u64 top = ~0ull;
+  for (uint32_t k = 0; k < K; ++k) {
+    u64 next = 0;                          // below every logit's key; 0 also where logits run out
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const u64 key = key_of(i);
+      if (key < top && key > next) next = key;
+    }
+    top = block_max(next);
+    if (threadIdx.x == 0) keys[k] = top;
   }
 }
 
@@ -137,8 +216,14 @@ __device__ __forceinline__ Cand shfl(const Cand& c, int o) {
 __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
   __shared__ double base[PVLC_BEAM_MAX_BEAMS];
   __shared__ Cand part[THREADS / 32];
-  const uint32_t r = blockIdx.x, W = p.beams;
+  __shared__ Cand list[LIST];
+  __shared__ Cand bound;
+  __shared__ uint32_t listed;
+  const uint32_t r = blockIdx.x, W = p.beams, K = p.topk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) listed = 0;
+  pdl_wait();
+  pdl_launch_dependents();
   for (uint32_t w = warp; w < W; w += THREADS / 32) {
     const float2* s = p.sums + (size_t)(r * W + w) * p.chunks;
     float m = -CUDART_INF_F;
@@ -146,28 +231,69 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     double t = 0.0;
     for (uint32_t c = lane; c < p.chunks; c += 32)
-      if (s[c].x > -CUDART_INF_F) t += (double)s[c].y * exp((double)s[c].x - (double)m);
+      if (s[c].x > -CUDART_INF_F) t += (double)s[c].y * (double)expf(s[c].x - m);
     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane == 0) base[w] = (double)p.scores[r * W + w] - ((double)m + log(t));
   }
   __syncthreads();
-  const uint32_t per = p.chunks * p.topk, n = W * per;
+  const uint32_t per = p.chunks * K, heads = W * p.chunks, n = W * per;
   const u64* keys = p.keys + (size_t)r * n;
+  auto candidate = [&](uint32_t i) {
+    Cand c;
+    c.key = keys[i];
+    c.beam = i / per;
+    c.score = base[c.beam] + (double)from_ordered((uint32_t)(c.key >> 32));
+    if (isnan(c.score)) c.score = -CUDART_INF;
+    return c;
+  };
+  auto write = [&](uint32_t k, const Cand& c) {
+    const size_t at = (size_t)r * K + k;
+    p.out_score[at] = (float)c.score;
+    p.out_beam[at] = (int32_t)c.beam;
+    p.out_token[at] = (int32_t)(0xffffffffu - (uint32_t)c.key);
+  };
+  // the K-th best of the chunks' best bounds the K best of all
+  const bool bounded = heads >= K && heads <= MAX_HEADS;
+  if (bounded) {
+    for (uint32_t i = threadIdx.x; i < heads; i += THREADS) list[i] = candidate(i * K);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < heads; i += THREADS) {
+      const Cand mine = list[i];
+      uint32_t rank = 0;
+      for (uint32_t j = 0; j < heads; ++j) rank += before(list[j], mine);
+      if (rank == K - 1) bound = mine;
+    }
+    __syncthreads();
+    const Cand b = bound;
+    for (uint32_t i = threadIdx.x; i < heads; i += THREADS)
+      for (uint32_t k = 0; k < K; ++k) {     // a chunk's list is in order
+        const Cand c = candidate(i * K + k);
+        if (c.key == 0 || before(b, c)) break;
+        const uint32_t at = atomicAdd(&listed, 1);
+        if (at < LIST) list[at] = c;
+      }
+    __syncthreads();
+    const uint32_t found = listed;
+    if (found <= LIST) {
+      for (uint32_t i = threadIdx.x; i < found; i += THREADS) {
+        const Cand mine = list[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < found; ++j) rank += before(list[j], mine);
+        if (rank < K) write(rank, mine);
+      }
+      return;
+    }
+  }
   Cand last;
   last.key = 0;
-  for (uint32_t k = 0; k < p.topk; ++k) {
+  for (uint32_t k = 0; k < K; ++k) {
     Cand best;
     best.key = 0;
     best.score = 0.0;
     best.beam = 0;
     for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-      Cand c;
-      c.key = keys[i];
-      if (c.key == 0) continue;
-      c.beam = i / per;
-      c.score = base[c.beam] + (double)from_ordered((uint32_t)(c.key >> 32));
-      if (isnan(c.score)) c.score = -CUDART_INF;
-      if ((k == 0 || before(last, c)) && before(c, best)) best = c;
+      const Cand c = candidate(i);
+      if (c.key != 0 && (k == 0 || before(last, c)) && before(c, best)) best = c;
     }
     for (int o = 16; o; o >>= 1) {
       const Cand y = shfl(best, o);
@@ -180,21 +306,40 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
     for (int i = 1; i < THREADS / 32; ++i)
       if (before(part[i], best)) best = part[i];
     last = best;
-    if (threadIdx.x == 0) {
-      const size_t at = (size_t)r * p.topk + k;
-      p.out_score[at] = (float)best.score;
-      p.out_beam[at] = (int32_t)best.beam;
-      p.out_token[at] = (int32_t)(0xffffffffu - (uint32_t)best.key);
-    }
+    if (threadIdx.x == 0) write(k, best);
   }
 }
 
-uint32_t chunks_of(uint32_t vocab) { return (vocab + CHUNK - 1) / CHUNK; }
+// Logits a thread: 32 keeps 13 chunks a row of a vocabulary of 10^5; few rows
+// get chunks of a quarter of that, so that they reach every SM.
+uint32_t per_thread(uint32_t rows, uint32_t beams, uint32_t vocab) {
+  const uint32_t wide = (vocab + THREADS * 32 - 1) / (THREADS * 32);
+  const uint32_t narrow = (vocab + THREADS * 8 - 1) / (THREADS * 8);
+  const bool few = (uint64_t)rows * wide < 2u * (uint32_t)sms_or_default_count();
+  return few && (uint64_t)beams * narrow <= MAX_HEADS ? 8 : 32;
+}
+uint32_t chunks_of(uint32_t rows, uint32_t beams, uint32_t vocab) {
+  const uint32_t chunk = THREADS * per_thread(rows, beams, vocab);
+  return (vocab + chunk - 1) / chunk;
+}
+
+template <typename T, bool VEC>
+cudaError_t launch_chunks(const Params& p, uint32_t per, const cudaLaunchConfig_t& cfg) {
+  return per == 8 ? cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, 8, VEC>, p)
+                  : cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, 32, VEC>, p);
+}
 
 }  // namespace beam
 
 size_t beam_topk_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t topk) {
-  const size_t slots = (size_t)batch * beams * beam::chunks_of(vocab);
+  // enough for every call of these sizes or smaller ones: fewer rows may have narrower chunks,
+  // at most 4 for each wide one, as long as those are below two an SM
+  const size_t rows = (size_t)batch * beams;
+  const size_t wide = (vocab + beam::THREADS * 32 - 1) / (beam::THREADS * 32);
+  const size_t narrow = (vocab + beam::THREADS * 8 - 1) / (beam::THREADS * 8);
+  const size_t few = 8 * (size_t)sms_or_default_count() + 4 * wide;
+  const size_t low = rows * narrow < few ? rows * narrow : few;
+  const size_t slots = rows * wide > low ? rows * wide : low;
   return (slots * (topk + 1) * 8 + 255) / 256 * 256;
 }
 
@@ -207,19 +352,33 @@ int beam_topk_launch(const BeamArgs& a, cudaStream_t stream) {
   p.beams = a.beams;
   p.vocab = a.vocab;
   p.topk = a.topk;
-  p.chunks = beam::chunks_of(a.vocab);
+  const uint32_t rows = a.batch * a.beams, per = beam::per_thread(rows, a.beams, a.vocab);
+  p.chunks = beam::chunks_of(rows, a.beams, a.vocab);
   p.keys = static_cast<beam::u64*>(a.workspace);
-  p.sums = reinterpret_cast<float2*>(p.keys + (size_t)a.batch * a.beams * p.chunks * a.topk);
+  p.sums = reinterpret_cast<float2*>(p.keys + (size_t)rows * p.chunks * a.topk);
   p.out_score = a.out_score;
   p.out_beam = a.out_beam;
   p.out_token = a.out_token;
-  const dim3 grid(p.chunks, a.batch * a.beams);
-  if (a.half_logits)
-    beam::beam_chunk_kernel<__half><<<grid, beam::THREADS, 0, stream>>>(p);
-  else
-    beam::beam_chunk_kernel<float><<<grid, beam::THREADS, 0, stream>>>(p);
-  beam::beam_join_kernel<<<a.batch, beam::THREADS, 0, stream>>>(p);
-  return cudaPeekAtLastError() == cudaSuccess ? PVLC_OK : PVLC_CUDA_ERROR;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.chunks, rows);
+  cfg.blockDim = dim3(beam::THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const bool vec = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 &&
+                   a.ld % (a.half_logits ? 8 : 4) == 0;
+  const cudaError_t e =
+      a.half_logits ? (vec ? beam::launch_chunks<__half, true>(p, per, cfg)
+                           : beam::launch_chunks<__half, false>(p, per, cfg))
+                    : (vec ? beam::launch_chunks<float, true>(p, per, cfg)
+                           : beam::launch_chunks<float, false>(p, per, cfg));
+  if (e != cudaSuccess) return PVLC_CUDA_ERROR;
+  cfg.gridDim = dim3(a.batch);
+  return cudaLaunchKernelEx(&cfg, beam::beam_join_kernel, p) == cudaSuccess ? PVLC_OK
+                                                                            : PVLC_CUDA_ERROR;
 }
 
 }  // namespace pvlc

@@ -156,6 +156,31 @@ def test_captured_and_reused_workspace(cuda_lib):
             assert torch.equal(a, b)
 
 
+def test_workspace_serves_smaller_calls(cuda_lib):
+    from pvlc_b200 import ops
+    rng = np.random.default_rng(7)
+    ws = ops.BeamWorkspace(25, 1, 103424, 8)
+    for B, W, V in ((25, 1, 103424), (22, 1, 103424), (3, 4, 60000), (1, 1, 40), (5, 5, 8192)):
+        x = rng.standard_normal((B * W, V)).astype(np.float32)
+        s = (-rng.random((B, W))).astype(np.float32)
+        got = ops.beam_topk(torch.from_numpy(x).cuda(), torch.from_numpy(s).cuda(), 8, ws)
+        want, gap = plain(x, s, 8)
+        assert gap > 2e-6
+        np.testing.assert_array_equal(got[2].cpu().numpy(), want[2])
+
+
+def test_many_reach_the_bound(cuda_lib):
+    """Chunks where more elements reach the selection's bound than are ranked at once, next
+    to ordinary ones, and more chunks than a join bounds by."""
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((8, 60000)).astype(np.float32)
+    x[:, 9000:11000] = 6.5
+    x[3, 30000:30700] = 7.0
+    check(x, (-rng.random((2, 4))).astype(np.float32), 24)
+    big = rng.standard_normal((2, 4_300_000)).astype(np.float32)
+    check(big, np.array([[-0.5, -0.25]], np.float32), 5)
+
+
 def test_wrapper_refusals(cuda_lib):
     from pvlc_b200 import abi, ops
     x, s = torch.zeros((8, 100), device="cuda"), torch.zeros((2, 4), device="cuda")
