@@ -14,11 +14,11 @@
 // request then joins the chunks: the rows' log-sums in f64, so that candidates
 // of two beams that differ by more than 1e-7 are told apart, and the K best.
 //
-// Selection: the K-th best of any disjoint groups' best elements is a bound that
-// at least K elements reach, so only what reaches it is looked at -- in a chunk,
-// the K-th best of a warp's 32 lane maxima; in a join, the K-th best of the
-// chunks' best -- a few dozen elements, which are ranked by counting.  Where too
-// many reach the bound (equal or masked logits) the K are taken one at a time.
+// Selection: of any disjoint groups' maxima the K-th largest is a bound that at
+// least K elements reach, so only what reaches it is looked at -- in a chunk, of
+// the maxima of 8 .. 64 groups of lanes; in a join, of the chunks' best -- a few
+// dozen elements, which are ranked by counting.  Where too many reach the bound
+// (equal or masked logits) the K are taken one at a time.
 // Keys are unique, so nothing depends on the order in which threads arrive.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -34,7 +34,10 @@ namespace beam {
 
 constexpr int THREADS = 256;
 constexpr uint32_t LIST = 512;               // elements ranked by counting
-constexpr uint32_t MAX_HEADS = 512;          // chunks of a request that a join bounds by
+constexpr uint32_t MAX_HEADS = 2 * THREADS;  // chunks of a request that a join bounds by
+#ifndef BEAM_PER
+#define BEAM_PER 32
+#endif
 
 typedef unsigned long long u64;
 
@@ -92,12 +95,31 @@ struct Params {
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
+// The K-th largest of x[0 .. n), K <= n, equal ones counting one each; all threads
+// get it.  x is padded with -infinity to a multiple of 4.
+__device__ __forceinline__ float kth_largest(const float* x, uint32_t n, uint32_t K, float* result) {
+  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+    const float mine = x[i];
+    uint32_t above = 0, equal_before = 0;
+    for (uint32_t j = 0; j < n; j += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(x + j);
+      above += (y.x > mine) + (y.y > mine) + (y.z > mine) + (y.w > mine);
+      equal_before += (y.x == mine && j < i) + (y.y == mine && j + 1 < i) +
+                      (y.z == mine && j + 2 < i) + (y.w == mine && j + 3 < i);
+    }
+    if (above + equal_before == K - 1) *result = mine;
+  }
+  __syncthreads();
+  return *result;
+}
+
 // PER logits a thread; VEC: rows are 16-byte aligned and read so.
 template <typename T, int PER, bool VEC>
-__global__ void __launch_bounds__(THREADS) beam_chunk_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, PER == 32 ? 4 : 6) beam_chunk_kernel(const Params p) {
   constexpr uint32_t CHUNK = THREADS * PER;
   constexpr int W = VEC ? 16 / sizeof(T) : 1;        // logits of one load
-  __shared__ float warp_top[THREADS / 32], warp_bound[THREADS / 32];
+  __shared__ __align__(16) float group_top[64];
+  __shared__ float bound_out;
   __shared__ u64 list[LIST];
   __shared__ uint32_t listed;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -107,59 +129,56 @@ __global__ void __launch_bounds__(THREADS) beam_chunk_kernel(const Params p) {
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
   // token of v[i]: loads of W neighbours, THREADS loads apart
   auto token = [&](int i) { return c * CHUNK + (i / W * THREADS + threadIdx.x) * W + i % W; };
-  float v[PER];
+  float v[PER];                            // a NaN counts as -infinity
   if (VEC && (c + 1) * CHUNK <= p.vocab) {
+    uint4 y[PER / W];
+#pragma unroll
+    for (int i = 0; i < PER / W; ++i) y[i] = __ldg(reinterpret_cast<const uint4*>(x + token(i * W)));
 #pragma unroll
     for (int i = 0; i < PER; i += W) {
-      const uint4 y = __ldg(reinterpret_cast<const uint4*>(x + token(i)));
       T z[W];
-      memcpy(z, &y, sizeof(T) * W);
+      memcpy(z, &y[i / W], sizeof(T) * W);
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[i + e] = to_float(z[e]);
+      for (int e = 0; e < W; ++e) v[i + e] = fmaxf(to_float(z[e]), -CUDART_INF_F);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const uint32_t at = token(i);
-      v[i] = at < p.vocab ? to_float(x[at]) : -CUDART_INF_F;
+      v[i] = at < p.vocab ? fmaxf(to_float(x[at]), -CUDART_INF_F) : -CUDART_INF_F;
     }
   }
-  float best = -CUDART_INF_F;
+  float best = v[0];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) best = fmaxf(best, v[i]);    // a NaN counts as -infinity
-  // lane maxima in descending order: the K-th is the warp's bound
-  float sorted = best;
+  for (int i = 1; i < PER; ++i) best = fmaxf(best, v[i]);
+  // groups of 32 lanes for K <= 8, .. of 4 lanes for K <= 64
+  const uint32_t split = K <= 8 ? 1 : K <= 16 ? 2 : K <= 32 ? 4 : 8, size = 32 / split;
 #pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j; j >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, sorted, j);
-      const bool up = ((lane & k) == 0) == ((lane & j) == 0);
-      sorted = up ? fmaxf(sorted, y) : fminf(sorted, y);
-    }
-  const float kth = __shfl_sync(0xffffffffu, sorted, K <= 32 ? K - 1 : 31);
-  if (lane == 0) {
-    warp_top[warp] = sorted;
-    warp_bound[warp] = kth;
+  for (uint32_t o = 1; o < 32; o <<= 1) {
+    const float y = __shfl_xor_sync(0xffffffffu, best, o);
+    if (o < size) best = fmaxf(best, y);
   }
+  if (lane % size == 0) group_top[warp * split + lane / size] = best;
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
-  float m = warp_top[0], bound = warp_bound[0];
-#pragma unroll
-  for (int w = 1; w < THREADS / 32; ++w) {
-    m = fmaxf(m, warp_top[w]);
-    bound = fmaxf(bound, warp_bound[w]);
+  const uint32_t groups = THREADS / 32 * split;
+  float m = -CUDART_INF_F;
+  for (uint32_t i = 0; i < groups; i += 4) {
+    const float4 y = *reinterpret_cast<const float4*>(group_top + i);
+    m = fmaxf(fmaxf(m, fmaxf(y.x, y.y)), fmaxf(y.z, y.w));
   }
   float s = 0.f;
+  if (m > -CUDART_INF_F) {                 // a masked token adds 2^-infinity
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    s += v[i] > -CUDART_INF_F ? exp2f((v[i] - m) * 1.4426950408889634f) : 0.f;
+    for (int i = 0; i < PER; ++i) s += fast_exp2((v[i] - m) * 1.4426950408889634f);
+  }
+  const float bound = kth_largest(group_top, groups, K, &bound_out);
   const size_t slot = (size_t)row * p.chunks + c;
   u64* keys = p.keys + slot * K;
   auto key_of = [&](int i) -> u64 {
     return token(i) < p.vocab ? (u64)ordered(v[i]) << 32 | (0xffffffffu - token(i)) : 0;
   };
-  if (K <= 32 && bound > -CUDART_INF_F) {
+  if (bound > -CUDART_INF_F) {
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (v[i] >= bound) {
@@ -217,69 +236,90 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
   __shared__ double base[PVLC_BEAM_MAX_BEAMS];
   __shared__ Cand part[THREADS / 32];
   __shared__ Cand list[LIST];
-  __shared__ Cand bound;
+  __shared__ __align__(16) float head_score[MAX_HEADS];
+  __shared__ float bound_out;
   __shared__ uint32_t listed;
   const uint32_t r = blockIdx.x, W = p.beams, K = p.topk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t per = p.chunks * K, heads = W * p.chunks, n = W * per;
+  const u64* keys = p.keys + (size_t)r * n;
+  const bool bounded = heads >= K && heads <= MAX_HEADS;
   if (threadIdx.x == 0) listed = 0;
   pdl_wait();
   pdl_launch_dependents();
+  // this thread's chunks' best, in flight under the log-sums
+  u64 mine[2] = {0, 0};
+  if (bounded) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (threadIdx.x + e * THREADS < heads) mine[e] = keys[(size_t)(threadIdx.x + e * THREADS) * K];
+  }
   for (uint32_t w = warp; w < W; w += THREADS / 32) {
     const float2* s = p.sums + (size_t)(r * W + w) * p.chunks;
+    const float score = p.scores[r * W + w];
     float m = -CUDART_INF_F;
-    for (uint32_t c = lane; c < p.chunks; c += 32) m = fmaxf(m, s[c].x);
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    double t = 0.0;
-    for (uint32_t c = lane; c < p.chunks; c += 32)
-      if (s[c].x > -CUDART_INF_F) t += (double)s[c].y * (double)expf(s[c].x - m);
+    double t = 0.0;                        // against m, rescaled where m grows
+    for (uint32_t c0 = 0; c0 < p.chunks; c0 += 32) {
+      const float2 x = c0 + lane < p.chunks ? s[c0 + lane] : make_float2(-CUDART_INF_F, 0.f);
+      float top = x.x;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (top > m) {
+        if (m > -CUDART_INF_F) t *= (double)expf(m - top);
+        m = top;
+      }
+      if (x.x > -CUDART_INF_F) t += (double)x.y * (double)expf(x.x - m);
+    }
+#pragma unroll
     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0) base[w] = (double)p.scores[r * W + w] - ((double)m + log(t));
+    if (lane == 0) base[w] = (double)score - ((double)m + log(t));
   }
   __syncthreads();
-  const uint32_t per = p.chunks * K, heads = W * p.chunks, n = W * per;
-  const u64* keys = p.keys + (size_t)r * n;
-  auto candidate = [&](uint32_t i) {
+  auto made = [&](u64 key, uint32_t beam) {
     Cand c;
-    c.key = keys[i];
-    c.beam = i / per;
-    c.score = base[c.beam] + (double)from_ordered((uint32_t)(c.key >> 32));
+    c.key = key;
+    c.beam = beam;
+    c.score = base[beam] + (double)from_ordered((uint32_t)(key >> 32));
     if (isnan(c.score)) c.score = -CUDART_INF;
     return c;
   };
+  auto candidate = [&](uint32_t i) { return made(keys[i], i / per); };
   auto write = [&](uint32_t k, const Cand& c) {
     const size_t at = (size_t)r * K + k;
     p.out_score[at] = (float)c.score;
     p.out_beam[at] = (int32_t)c.beam;
     p.out_token[at] = (int32_t)(0xffffffffu - (uint32_t)c.key);
   };
-  // the K-th best of the chunks' best bounds the K best of all
-  const bool bounded = heads >= K && heads <= MAX_HEADS;
   if (bounded) {
-    for (uint32_t i = threadIdx.x; i < heads; i += THREADS) list[i] = candidate(i * K);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < heads; i += THREADS) {
-      const Cand mine = list[i];
-      uint32_t rank = 0;
-      for (uint32_t j = 0; j < heads; ++j) rank += before(list[j], mine);
-      if (rank == K - 1) bound = mine;
+    // scores rounded down to f32: at least K chunks' best reach the K-th largest of them
+    float score[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t i = threadIdx.x + e * THREADS;
+      score[e] = i < heads ? __double2float_rd(made(mine[e], i / p.chunks).score) : -CUDART_INF_F;
+      head_score[i] = score[e];
     }
     __syncthreads();
-    const Cand b = bound;
-    for (uint32_t i = threadIdx.x; i < heads; i += THREADS)
+    const float bound = kth_largest(head_score, heads, K, &bound_out);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t i = threadIdx.x + e * THREADS;
+      if (i >= heads || !(score[e] >= bound)) continue;
       for (uint32_t k = 0; k < K; ++k) {     // a chunk's list is in order
         const Cand c = candidate(i * K + k);
-        if (c.key == 0 || before(b, c)) break;
+        if (c.key == 0 || c.score < (double)bound) break;
         const uint32_t at = atomicAdd(&listed, 1);
         if (at < LIST) list[at] = c;
       }
+    }
     __syncthreads();
     const uint32_t found = listed;
     if (found <= LIST) {
       for (uint32_t i = threadIdx.x; i < found; i += THREADS) {
-        const Cand mine = list[i];
+        const Cand c = list[i];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < found; ++j) rank += before(list[j], mine);
-        if (rank < K) write(rank, mine);
+        for (uint32_t j = 0; j < found; ++j) rank += before(list[j], c);
+        if (rank < K) write(rank, c);
       }
       return;
     }
@@ -313,10 +353,10 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
 // Logits a thread: 32 keeps 13 chunks a row of a vocabulary of 10^5; few rows
 // get chunks of a quarter of that, so that they reach every SM.
 uint32_t per_thread(uint32_t rows, uint32_t beams, uint32_t vocab) {
-  const uint32_t wide = (vocab + THREADS * 32 - 1) / (THREADS * 32);
+  const uint32_t wide = (vocab + THREADS * BEAM_PER - 1) / (THREADS * BEAM_PER);
   const uint32_t narrow = (vocab + THREADS * 8 - 1) / (THREADS * 8);
   const bool few = (uint64_t)rows * wide < 2u * (uint32_t)sms_or_default_count();
-  return few && (uint64_t)beams * narrow <= MAX_HEADS ? 8 : 32;
+  return few && (uint64_t)beams * narrow <= MAX_HEADS ? 8 : BEAM_PER;
 }
 uint32_t chunks_of(uint32_t rows, uint32_t beams, uint32_t vocab) {
   const uint32_t chunk = THREADS * per_thread(rows, beams, vocab);
@@ -326,7 +366,7 @@ uint32_t chunks_of(uint32_t rows, uint32_t beams, uint32_t vocab) {
 template <typename T, bool VEC>
 cudaError_t launch_chunks(const Params& p, uint32_t per, const cudaLaunchConfig_t& cfg) {
   return per == 8 ? cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, 8, VEC>, p)
-                  : cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, 32, VEC>, p);
+                  : cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, BEAM_PER, VEC>, p);
 }
 
 }  // namespace beam
@@ -335,7 +375,7 @@ size_t beam_topk_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab,
   // enough for every call of these sizes or smaller ones: fewer rows may have narrower chunks,
   // at most 4 for each wide one, as long as those are below two an SM
   const size_t rows = (size_t)batch * beams;
-  const size_t wide = (vocab + beam::THREADS * 32 - 1) / (beam::THREADS * 32);
+  const size_t wide = (vocab + beam::THREADS * BEAM_PER - 1) / (beam::THREADS * BEAM_PER);
   const size_t narrow = (vocab + beam::THREADS * 8 - 1) / (beam::THREADS * 8);
   const size_t few = 8 * (size_t)sms_or_default_count() + 4 * wide;
   const size_t low = rows * narrow < few ? rows * narrow : few;
