@@ -8,21 +8,17 @@
 // the lower token.  Within a beam the order is that of the logits, so each
 // row's K best logits are enough, and they need no logarithm.
 //
-// One pass over the logits, bound by HBM: all rows' chunks of 8192 are laid end
-// to end and cut into equal ranges, one per block.  A block's threads each
-// stream their own 32 logits of a chunk through two cp.async stages, keep a running maximum and sum of exponentials, and push what may be among the
-// K best of the row into a list.  Per part of a row the block leaves its sum and
-// its K best logits as 64-bit keys (ordered logit, then ~token), best first.  A
-// block per request joins the parts: the rows' log-sums in f64, so that candidates
+// One pass over the logits, bound by HBM: a block holds a chunk of a row in
+// registers, sums its exponentials against its own maximum and keeps its K best
+// logits as 64-bit keys (ordered logit, then ~token), best first.  A block per
+// request then joins the chunks: the rows' log-sums in f64, so that candidates
 // of two beams that differ by more than 1e-7 are told apart, and the K best.
 //
 // Selection: of any disjoint groups' maxima the K-th largest is a bound that at
-// least K elements reach, so only what reaches it is looked at -- in a row's first
-// chunk (and in one that raises the level), of the maxima of 8 .. 64 groups of
-// lanes; in a join, of the parts' best -- a few dozen elements, which are ranked
-// by counting.  A ranked list's K-th key is the bound of the chunks that follow.
-// Where too many reach the bound (equal or masked logits) the K are taken one at
-// a time.
+// least K elements reach, so only what reaches it is looked at -- in a chunk, of
+// the maxima of 64 groups of 4 lanes; in a join, of the chunks' best -- a few
+// dozen elements, which are ranked by counting.  Where too many reach the bound
+// (equal or masked logits) the K are taken one at a time.
 // Keys are unique, so nothing depends on the order in which threads arrive.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,11 +33,9 @@ namespace pvlc {
 namespace beam {
 
 constexpr int THREADS = 256;
-constexpr int PER = 32;                      // logits of a chunk a thread (and a warp's lanes)
-constexpr uint32_t CHUNK = THREADS * PER;
-constexpr int BLOCKS = 3;                    // of an SM
 constexpr uint32_t LIST = 512;               // elements ranked by counting
-constexpr uint32_t MAX_HEADS = 2 * THREADS;  // parts of a request that a join bounds by
+constexpr uint32_t MAX_HEADS = 2 * THREADS;  // chunks of a request that a join bounds by
+constexpr int BLOCKS = 5;                    // of an SM
 
 typedef unsigned long long u64;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -72,30 +66,13 @@ __device__ __forceinline__ u64 block_max(u64 v) {
   return r;
 }
 
-__device__ __forceinline__ float block_sum(float v) {
-  __shared__ float part[THREADS / 32];
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = 0.f;
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) r += part[i];
-  return r;
-}
-
 struct Params {
   const void* logits;
   uint64_t ld;
   const float* scores;
-  uint32_t batch, beams, vocab, topk;
-  uint32_t chunks;    // of a row
-  uint32_t blocks;    // of the chunk kernel
-  uint32_t parts;     // most blocks that share a row
-  u64* keys;          // [rows][parts][topk]
-  float2* sums;       // [rows][parts] (maximum, sum of exponentials against it)
-  uint32_t* counts;   // [rows] how many parts the row has
+  uint32_t batch, beams, vocab, topk, chunks;
+  u64* keys;          // [rows][chunks][topk]
+  float2* sums;       // [rows][chunks] (maximum, sum of exponentials against it)
   float* out_score;
   int32_t* out_beam;
   int32_t* out_token;
@@ -127,245 +104,143 @@ __device__ __forceinline__ float kth_largest(const float* x, uint32_t n, uint32_
   return *result;
 }
 
-// Block i's chunks are [cut(i), cut(i + 1)) of the rows' chunks end to end.
-__host__ __device__ __forceinline__ uint64_t cut(const Params& p, uint64_t i) {
-  const uint64_t x = i * ((uint64_t)p.batch * p.beams * p.chunks);
-  return x >> 32 ? x / p.blocks : (uint32_t)x / p.blocks;
-}
-// The block that holds chunk u.
-__device__ __forceinline__ uint32_t block_of(const Params& p, uint64_t u) {
-  const uint64_t n = (uint64_t)p.batch * p.beams * p.chunks, x = (u + 1) * p.blocks + n - 1;
-  return (uint32_t)(x >> 32 ? x / n : (uint32_t)x / (uint32_t)n) - 1;
-}
-
-// VEC: rows are 16-byte aligned.
-template <typename T, bool VEC>
+// PER logits a thread; VEC: rows are 16-byte aligned.
+template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(THREADS, BLOCKS) beam_chunk_kernel(const Params p) {
-  constexpr int W = 16 / sizeof(T);                  // logits of one 16-byte piece
-  constexpr int PIECES = PER / W;
-  extern __shared__ __align__(16) uint8_t ring[];    // [2][PIECES][THREADS] x 16 bytes
-  __shared__ __align__(16) float group_top[64];
+  constexpr uint32_t CHUNK = THREADS * PER;
+  constexpr uint32_t W = 16 / sizeof(T);             // logits of one 16-byte load
+  constexpr uint32_t GROUPS = THREADS / 4;           // of 4 lanes
+  __shared__ __align__(16) float group_top[GROUPS];
+  __shared__ float2 warp_sum[THREADS / 32];
   __shared__ float bound_out;
   __shared__ u64 list[LIST];
-  __shared__ u64 best_keys[PVLC_BEAM_MAX_TOPK];
+  __shared__ __align__(16) float handed[THREADS / 32][PER];
   __shared__ uint32_t listed;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t K = p.topk;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_launch_dependents();
-  const uint64_t u0 = cut(p, blockIdx.x), u1 = cut(p, blockIdx.x + 1);
-  // v[i] of chunk c is token(c, i): pieces of W neighbours, THREADS pieces apart
-  auto token = [&](uint32_t c, int i) { return c * CHUNK + (i / W * THREADS + tid) * W + i % W; };
-  uint32_t next_row = (uint32_t)(u0 / p.chunks), next_chunk = (uint32_t)(u0 % p.chunks);
-  uint64_t next = u0;
-  // Start this thread's copies of the next chunk.  Only the thread itself reads them.
-  auto fetch = [&](uint32_t stage) {
-    if (next < u1) {
-      const T* x = static_cast<const T*>(p.logits) + next_row * p.ld;
+  const uint32_t row = blockIdx.y, c = blockIdx.x, K = p.topk;
+  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+  // logit i of thread t is token(t, i): w neighbours a load, THREADS loads apart
+  const uint32_t w = VEC && (c + 1) * CHUNK <= p.vocab ? W : 1;
+  auto token = [&](uint32_t t, uint32_t i) { return c * CHUNK + (i / w * THREADS + t) * w + i % w; };
+  float v[PER];
+  if (w == W) {
+    uint4 y[PER / W];
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        uint8_t* to = ring + ((stage * PIECES + i) * THREADS + tid) * 16;
-        const uint32_t at = token(next_chunk, i * W);
-        if (VEC && at + W <= p.vocab) {
-          cp_async_16(smem_u32(to), x + at);
-        } else {
+    for (uint32_t i = 0; i < PER / W; ++i)
+      y[i] = __ldg(reinterpret_cast<const uint4*>(x + c * CHUNK + (i * THREADS + tid) * W));
 #pragma unroll
-          for (int e = 0; e < W; ++e)    // behind the row: masked
-            reinterpret_cast<T*>(to)[e] = at + e < p.vocab ? x[at + e] : T(-CUDART_INF_F);
-        }
-      }
-      if (++next_chunk == p.chunks) {
-        next_chunk = 0;
-        ++next_row;
-      }
-      ++next;
+    for (uint32_t i = 0; i < PER; i += W) {
+      T z[W];
+      memcpy(z, &y[i / W], sizeof(T) * W);
+#pragma unroll
+      for (uint32_t e = 0; e < W; ++e) v[i + e] = to_float(z[e]);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  fetch(0);
-
-  uint32_t row = (uint32_t)(u0 / p.chunks), c = (uint32_t)(u0 % p.chunks), stage = 0;
-  uint32_t from = c;                     // the row's first chunk in this block
-  float m = -CUDART_INF_F, s = 0.f;      // this thread's, of the row so far
-  u64 bound = 0;                         // only larger keys matter
-  uint32_t kept = 0;                     // keys in the list, at most LIST / 4
-  bool first = true;
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+      const uint32_t at = c * CHUNK + i * THREADS + tid;
+      v[i] = at < p.vocab ? to_float(x[at]) : -CUDART_INF_F;
+    }
+  }
   if (tid == 0) listed = 0;
+  float best = -CUDART_INF_F;                // the maxima pass over NaN
+#pragma unroll
+  for (int i = 0; i < PER; i += 2) best = fmax3(best, v[i], v[i + 1]);
+  // ---- the warp's maximum and its sum of exponentials
+  float m = best;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (o == 2 && lane % 4 == 0) group_top[tid / 4] = m;
+  }
+  float s = 0.f;
+  if (m > -CUDART_INF_F) {                   // a masked token adds 2^-infinity
+    const uint64_t shift = f2_pack(-m, -m), unit = f2_pack(kLog2e, kLog2e);
+    uint64_t sum = f2_pack(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) {
+      const float2 y = f2_unpack(f2_mul(f2_add(f2_pack(v[i], v[i + 1]), shift), unit));
+      sum = f2_add(sum, f2_pack(fast_exp2(y.x), fast_exp2(y.y)));
+    }
+    const float2 both = f2_unpack(sum);
+    s = both.x + both.y;
+    if (isnan(s) && m < CUDART_INF_F) {      // a NaN counts as -infinity
+      s = 0.f;
+#pragma unroll 1
+      for (uint32_t i = 0; i < PER; ++i) {
+        const float y = token(tid, i) < p.vocab ? to_float(x[token(tid, i)]) : -CUDART_INF_F;
+        if (y > -CUDART_INF_F) s += fast_exp2((y - m) * kLog2e);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) warp_sum[warp] = make_float2(m, s);
   __syncthreads();
-  // The list's K best, in order, become the list; the K-th is the bound.
-  auto rank_list = [&]() {
-    const uint32_t n = listed;           // at most LIST
+  // ---- what reaches the K-th largest group maximum
+  const size_t slot = (size_t)row * p.chunks + c;
+  u64* keys = p.keys + slot * K;
+  const float bound = kth_largest(group_top, GROUPS, K, &bound_out);
+  auto key_of = [](float y, uint32_t at) -> u64 { return (u64)ordered(y) << 32 | (0xffffffffu - at); };
+  if (bound > -CUDART_INF_F) {
+    // The warp looks at each thread that has something together, one of its logits a lane,
+    // handed over through shared memory: as unrolled code on registers this rare work took
+    // longer to fetch than to run.
+    uint32_t found = __ballot_sync(0xffffffffu, best >= bound);
+    while (found) {
+      const uint32_t who = __ffs(found) - 1;
+      found &= found - 1;
+      if (lane == who) {
+#pragma unroll
+        for (int i = 0; i < PER; i += 4)
+          *reinterpret_cast<float4*>(handed[warp] + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      }
+      __syncwarp();
+      const float y = lane < PER ? handed[warp][lane] : -CUDART_INF_F;
+      if (y >= bound) {
+        const uint32_t to = atomicAdd(&listed, 1);
+        if (to < LIST) list[to] = key_of(y, token(warp * 32 + who, lane));
+      }
+      __syncwarp();
+    }
+  } else if (tid == 0) {
+    listed = LIST + 1;                       // fewer than K groups hold anything
+  }
+  __syncthreads();
+  if (tid == 0) {
+    float2 all = warp_sum[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) all.x = fmaxf(all.x, warp_sum[i].x);
+    all.y = 0.f;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i)
+      if (warp_sum[i].x > -CUDART_INF_F) all.y += warp_sum[i].y * fast_exp2((warp_sum[i].x - all.x) * kLog2e);
+    p.sums[slot] = all;
+  }
+  const uint32_t n = listed;
+  if (n <= LIST) {
     for (uint32_t i = tid; i < n; i += THREADS) {
       const u64 mine = list[i];
       uint32_t rank = 0;
       for (uint32_t j = 0; j < n; ++j) rank += list[j] > mine;
-      if (rank < K) best_keys[rank] = mine;
+      if (rank < K) keys[rank] = mine;
     }
-    __syncthreads();
-    kept = n < K ? n : K;
-    for (uint32_t i = tid; i < kept; i += THREADS) list[i] = best_keys[i];
-    if (tid == 0) listed = kept;
-    if (kept == K) bound = best_keys[K - 1];
-    __syncthreads();
-  };
-  for (uint64_t u = u0; u < u1; ++u) {
-    fetch(stage ^ 1);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    float v[PER];
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint4 y = reinterpret_cast<const uint4*>(ring)[(stage * PIECES + i) * THREADS + tid];
-      T z[W];
-      memcpy(z, &y, 16);
-#pragma unroll
-      for (int e = 0; e < W; ++e) v[i * W + e] = to_float(z[e]);
-    }
-    float best = -CUDART_INF_F;          // the maxima pass over NaN
-#pragma unroll
-    for (int i = 0; i < PER; i += 2) best = fmax3(best, v[i], v[i + 1]);
-    if (best > m) {
-      s *= fast_exp2((m - best) * kLog2e);
-      m = best;
-    }
-    if (m > -CUDART_INF_F) {             // a masked token adds 2^-infinity
-      const uint64_t shift = f2_pack(-m, -m), unit = f2_pack(kLog2e, kLog2e);
-      uint64_t sum = f2_pack(s, 0.f);
-#pragma unroll
-      for (int i = 0; i < PER; i += 2) {
-        const float2 x = f2_unpack(f2_mul(f2_add(f2_pack(v[i], v[i + 1]), shift), unit));
-        sum = f2_add(sum, f2_pack(fast_exp2(x.x), fast_exp2(x.y)));
-      }
-      const float2 both = f2_unpack(sum);
-      s = both.x + both.y;
-    }
-    // The rare work on single logits reads them again: the code stays small, and with
-    // it the time to fetch its instructions (unrolled, it cost 5 us a chunk).
-    const uint32_t now = stage;
-    auto each = [&](auto f) {              // f(ordered logit, token)
-#pragma unroll 1
-      for (int i = 0; i < PIECES; ++i) {
-        const uint4 y = reinterpret_cast<const uint4*>(ring)[(now * PIECES + i) * THREADS + tid];
-        const uint32_t at = token(c, i * W);
-        T z[W];
-        memcpy(z, &y, 16);
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          if (at + e < p.vocab) f(to_float(z[e]), at + e);
-      }
-    };
-    auto key_of = [](float x, uint32_t at) -> u64 { return (u64)ordered(x) << 32 | (0xffffffffu - at); };
-    // a float that every key above the bound reaches (0 bounds nothing)
-    const float level = bound ? from_ordered((uint32_t)(bound >> 32)) : -CUDART_INF_F;
-    const int reach = __syncthreads_count(best >= level && (best > -CUDART_INF_F || bound == 0));
-    if (reach) {
-      bool singly = false;
-      u64 bar = bound;
-      if (reach > THREADS / 4) {
-        // raise the bound by this chunk's groups: 32 lanes for K <= 8, .. 4 lanes for K <= 64
-        const uint32_t split = K <= 8 ? 1 : K <= 16 ? 2 : K <= 32 ? 4 : 8, size = 32 / split;
-        float top = best;
-#pragma unroll
-        for (uint32_t o = 1; o < 32; o <<= 1) {
-          const float y = __shfl_xor_sync(0xffffffffu, top, o);
-          if (o < size) top = fmaxf(top, y);
-        }
-        if (lane % size == 0) group_top[warp * split + lane / size] = top;
-        __syncthreads();
-        const float kth = kth_largest(group_top, THREADS / 32 * split, K, &bound_out);
-        if (kth > -CUDART_INF_F) {
-          const u64 key = ((u64)ordered(kth) << 32) - 1;
-          bar = key > bar ? key : bar;
-        } else {
-          singly = true;                 // fewer than K groups hold anything
-        }
-      }
-      if (!singly) {
-        const float lowest = bar ? from_ordered((uint32_t)(bar >> 32)) : -CUDART_INF_F;
-        // the warp looks at each such thread's logits together, one a lane
-        uint32_t found = __ballot_sync(0xffffffffu, best >= lowest);
-        while (found) {
-          const int who = warp * 32 + __ffs(found) - 1;
-          found &= found - 1;
-          const int piece = lane / W;
-          const uint32_t at = c * CHUNK + (piece * THREADS + who) * W + lane % W;
-          const float x = to_float(reinterpret_cast<const T*>(
-              ring + ((now * PIECES + piece) * THREADS + who) * 16)[lane % W]);
-          if (x >= lowest && at < p.vocab) {
-            const u64 key = key_of(x, at);
-            if (key > bar) {
-              const uint32_t to = atomicAdd(&listed, 1);
-              if (to < LIST) list[to] = key;
-            }
-          }
-        }
-        __syncthreads();
-        singly = listed > LIST;
-      }
-      if (singly) {
-        // too many: this chunk's K best one by one behind the row's
-        u64 top = ~0ull;
-        uint32_t n = kept;
-        for (uint32_t k = 0; k < K; ++k) {
-          u64 after = 0;                 // 0: the chunk's logits have run out
-          each([&](float x, uint32_t at) {
-            const u64 key = key_of(x, at);
-            if (key < top && key > after) after = key;
-          });
-          top = block_max(after);
-          if (top <= bound) break;
-          if (tid == 0) list[n] = top;
-          ++n;
-        }
-        if (tid == 0) listed = n;
-        __syncthreads();
-      }
-      kept = listed;
-      if (first || kept > LIST / 4) rank_list();
-      first = false;
-    }
-    stage ^= 1;
-    if (++c == p.chunks || u + 1 == u1) {
-      // ------------------------------------------- the part's record
-      rank_list();
-      float top = m;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (lane == 0) group_top[warp] = top;
-      __syncthreads();
-      top = group_top[0];
-#pragma unroll
-      for (int w = 1; w < THREADS / 32; ++w) top = fmaxf(top, group_top[w]);
-      float sum = block_sum(m > -CUDART_INF_F ? s * fast_exp2((m - top) * kLog2e) : 0.f);
-      if (isnan(sum) && top < CUDART_INF_F) {
-        // NaN among the logits: they count as -infinity, so sum the part again without them
-        s = 0.f;
-        const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-#pragma unroll 1
-        for (uint32_t at = from * CHUNK + tid; at < min(c * CHUNK, p.vocab); at += THREADS)
-          if (to_float(x[at]) > -CUDART_INF_F) s += fast_exp2((to_float(x[at]) - top) * kLog2e);
-        sum = block_sum(s);
-      }
-      const uint32_t part = blockIdx.x - block_of(p, (uint64_t)row * p.chunks);
-      const size_t slot = (size_t)row * p.parts + part;
-      if (tid == 0) {
-        p.sums[slot] = make_float2(top, sum);
-        if (c == p.chunks) p.counts[row] = part + 1;
-      }
-      const uint32_t n = listed;
-      for (uint32_t k = tid; k < K; k += THREADS) p.keys[slot * K + k] = k < n ? list[k] : 0;
-      __syncthreads();
-      if (tid == 0) listed = 0;
-      __syncthreads();
-      kept = 0;
-      m = -CUDART_INF_F;
-      s = 0.f;
-      bound = 0;
-      first = true;
-      c = from = 0;
-      ++row;
-    }
+    return;
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  u64 top = ~0ull;
+  for (uint32_t k = 0; k < K; ++k) {
+    u64 next = 0;                            // below every logit's key; 0 also where logits run out
+#pragma unroll 8
+    for (uint32_t i = 0; i < PER; ++i) {
+      const uint32_t at = token(tid, i);
+      const u64 key = at < p.vocab ? key_of(to_float(x[at]), at) : 0;
+      if (key < top && key > next) next = key;
+    }
+    top = block_max(next);
+    if (tid == 0) keys[k] = top;
+  }
 }
 
 struct Cand {
@@ -396,31 +271,29 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
   __shared__ uint32_t listed;
   const uint32_t r = blockIdx.x, W = p.beams, K = p.topk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t P = p.parts, heads = W * P;          // at most MAX_HEADS
-  const u64* keys = p.keys + (size_t)r * heads * K;
-  __shared__ uint32_t parts[PVLC_BEAM_MAX_BEAMS];    // that each row has
+  const uint32_t per = p.chunks * K, heads = W * p.chunks, n = W * per;
+  const u64* keys = p.keys + (size_t)r * n;
+  const bool bounded = heads >= K && heads <= MAX_HEADS;
   if (threadIdx.x == 0) listed = 0;
   pdl_wait();
   pdl_launch_dependents();
-  // this thread's parts' first keys (of parts that are there or not), in flight under the log-sums
-  constexpr uint32_t EARLY = 4;
+  // this thread's chunks' first keys, in flight under the log-sums
+  constexpr uint32_t EARLY = 2;
   u64 mine[2][EARLY];
 #pragma unroll
   for (int e = 0; e < 2; ++e)
 #pragma unroll
     for (uint32_t k = 0; k < EARLY; ++k) {
       const uint32_t i = threadIdx.x + e * THREADS;
-      mine[e][k] = i < heads && k < K ? keys[(size_t)i * K + k] : 0;
+      mine[e][k] = bounded && i < heads && k < K ? keys[(size_t)i * K + k] : 0;
     }
   for (uint32_t w = warp; w < W; w += THREADS / 32) {
-    const float2* s = p.sums + (size_t)(r * W + w) * P;
-    const float2 lead = lane < P ? s[lane] : make_float2(0.f, 0.f);
-    const uint32_t count = p.counts[r * W + w];
+    const float2* s = p.sums + (size_t)(r * W + w) * p.chunks;
     const float score = p.scores[r * W + w];
     float m = -CUDART_INF_F;
     double t = 0.0;                        // against m, rescaled where m grows
-    for (uint32_t c0 = 0; c0 < count; c0 += 32) {
-      const float2 x = c0 + lane < count ? (c0 ? s[c0 + lane] : lead) : make_float2(-CUDART_INF_F, 0.f);
+    for (uint32_t c0 = 0; c0 < p.chunks; c0 += 32) {
+      const float2 x = c0 + lane < p.chunks ? s[c0 + lane] : make_float2(-CUDART_INF_F, 0.f);
       float top = x.x;
 #pragma unroll
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -432,13 +305,9 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0) {
-      base[w] = (double)score - ((double)m + log(t));
-      parts[w] = count;
-    }
+    if (lane == 0) base[w] = (double)score - ((double)m + log(t));
   }
   __syncthreads();
-  auto there = [&](uint32_t i) { return i < heads && i % P < parts[i / P]; };   // part i of the request
   auto made = [&](u64 key, uint32_t beam) {
     Cand c;
     c.key = key;
@@ -447,51 +316,50 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
     if (isnan(c.score)) c.score = -CUDART_INF;
     return c;
   };
-  // candidate k of part i
-  auto candidate = [&](uint32_t i, uint32_t k) { return made(keys[(size_t)i * K + k], i / P); };
+  auto candidate = [&](uint32_t i) { return made(keys[i], i / per); };
   auto write = [&](uint32_t k, const Cand& c) {
     const size_t at = (size_t)r * K + k;
     p.out_score[at] = (float)c.score;
     p.out_beam[at] = (int32_t)c.beam;
     p.out_token[at] = (int32_t)(0xffffffffu - (uint32_t)c.key);
   };
-  // scores rounded down to f32: at least K parts' best reach the K-th largest of them (where
-  // there are fewer parts it is -infinity, and everything does)
-  float score[2];
+  if (bounded) {
+    // scores rounded down to f32: at least K chunks' best reach the K-th largest of them
+    float score[2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const uint32_t i = threadIdx.x + e * THREADS;
-    score[e] = there(i) ? __double2float_rd(made(mine[e][0], i / P).score) : -CUDART_INF_F;
-    head_score[i] = score[e];
-  }
-  __syncthreads();
-  const float bound =
-      heads >= K ? kth_largest(head_score, heads, K, &bound_out) : -CUDART_INF_F;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const uint32_t i = threadIdx.x + e * THREADS;
-    if (!there(i) || !(score[e] >= bound)) continue;
-    auto add = [&](const Cand& c) {          // a part's list is in order: false behind the last
-      if (c.key == 0 || c.score < (double)bound) return false;
-      const uint32_t at = atomicAdd(&listed, 1);
-      if (at < LIST) list[at] = c;
-      return true;
-    };
-    bool more = true;
-#pragma unroll
-    for (uint32_t k = 0; k < EARLY; ++k) more = more && add(made(mine[e][k], i / P));
-    for (uint32_t k = EARLY; k < K && more; ++k) more = add(candidate(i, k));
-  }
-  __syncthreads();
-  const uint32_t found = listed;
-  if (found <= LIST) {
-    for (uint32_t i = threadIdx.x; i < found; i += THREADS) {
-      const Cand c = list[i];
-      uint32_t rank = 0;
-      for (uint32_t j = 0; j < found; ++j) rank += before(list[j], c);
-      if (rank < K) write(rank, c);
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t i = threadIdx.x + e * THREADS;
+      score[e] = i < heads ? __double2float_rd(made(mine[e][0], i / p.chunks).score) : -CUDART_INF_F;
+      head_score[i] = score[e];
     }
-    return;
+    __syncthreads();
+    const float bound = kth_largest(head_score, heads, K, &bound_out);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t i = threadIdx.x + e * THREADS;
+      if (i >= heads || !(score[e] >= bound)) continue;
+      auto add = [&](const Cand& c) {        // a chunk's list is in order: false behind the last
+        if (c.key == 0 || c.score < (double)bound) return false;
+        const uint32_t at = atomicAdd(&listed, 1);
+        if (at < LIST) list[at] = c;
+        return true;
+      };
+      bool more = true;
+#pragma unroll
+      for (uint32_t k = 0; k < EARLY; ++k) more = more && add(made(mine[e][k], i / p.chunks));
+      for (uint32_t k = EARLY; k < K && more; ++k) more = add(candidate(i * K + k));
+    }
+    __syncthreads();
+    const uint32_t found = listed;
+    if (found <= LIST) {
+      for (uint32_t i = threadIdx.x; i < found; i += THREADS) {
+        const Cand c = list[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < found; ++j) rank += before(list[j], c);
+        if (rank < K) write(rank, c);
+      }
+      return;
+    }
   }
   Cand last;
   last.key = 0;
@@ -500,9 +368,8 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
     best.key = 0;
     best.score = 0.0;
     best.beam = 0;
-    for (uint32_t i = threadIdx.x; i < heads * K; i += THREADS) {
-      if (!there(i / K)) continue;
-      const Cand c = candidate(i / K, i % K);
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+      const Cand c = candidate(i);
       if (c.key != 0 && (k == 0 || before(last, c)) && before(c, best)) best = c;
     }
     for (int o = 16; o; o >>= 1) {
@@ -520,45 +387,37 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
   }
 }
 
-// How the rows' chunks are shared out: BLOCKS blocks an SM, or fewer where a
-// request would get more parts than its join can bound by.
-void share(Params& p) {
-  const uint64_t rows = (uint64_t)p.batch * p.beams;
-  p.chunks = (p.vocab + CHUNK - 1) / CHUNK;
-  const uint64_t units = rows * p.chunks;
-  uint64_t blocks = (uint64_t)BLOCKS * sms_or_default_count();
-  if (blocks > units) blocks = units;
-  while (true) {
-    const uint64_t q = units / blocks;             // every block has that many chunks or more
-    const uint64_t parts = (p.chunks - 1) / q + 2;
-    p.parts = (uint32_t)(parts < p.chunks ? parts : p.chunks);
-    if (p.parts * p.beams <= MAX_HEADS) break;
-    blocks = blocks * 7 / 8;                       // at `rows` blocks a row has 2 parts at most
-  }
-  p.blocks = (uint32_t)blocks;
+// Logits a thread: 32 keeps 13 chunks a row of a vocabulary of 10^5; few rows
+// get chunks of a quarter of that, so that they reach every SM.
+uint32_t per_thread(uint32_t rows, uint32_t beams, uint32_t vocab) {
+  const uint32_t wide = (vocab + THREADS * 32 - 1) / (THREADS * 32);
+  const uint32_t narrow = (vocab + THREADS * 8 - 1) / (THREADS * 8);
+  const bool few = (uint64_t)rows * wide < 2u * (uint32_t)sms_or_default_count();
+  return few && (uint64_t)beams * narrow <= MAX_HEADS ? 8 : 32;
+}
+uint32_t chunks_of(uint32_t rows, uint32_t beams, uint32_t vocab) {
+  const uint32_t chunk = THREADS * per_thread(rows, beams, vocab);
+  return (vocab + chunk - 1) / chunk;
 }
 
 template <typename T, bool VEC>
-int launch_chunks(const Params& p, cudaLaunchConfig_t cfg) {
-  cfg.gridDim = dim3(p.blocks);
-  cfg.dynamicSmemBytes = 2 * CHUNK * sizeof(T);
-  const void* fn = reinterpret_cast<const void*>(beam_chunk_kernel<T, VEC>);
-  if (const int st = set_smem_attribute_once(fn, 2 * CHUNK * sizeof(T))) return st;
-  return cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, VEC>, p) == cudaSuccess ? PVLC_OK
-                                                                                : PVLC_CUDA_ERROR;
+cudaError_t launch_chunks(const Params& p, uint32_t per, const cudaLaunchConfig_t& cfg) {
+  return per == 8 ? cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, 8, VEC>, p)
+                  : cudaLaunchKernelEx(&cfg, beam_chunk_kernel<T, 32, VEC>, p);
 }
 
 }  // namespace beam
 
 size_t beam_topk_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t topk) {
-  // Enough for every call of these sizes or smaller ones: rows x parts is at most rows x chunks,
-  // and at most 2 BLOCKS an SM and 2 a row (every block has a chunk; where it has q >= 2, a row has
-  // chunks / q + 2 parts and chunks / q is below 3 / 2 of the blocks per row).
+  // enough for every call of these sizes or smaller ones: fewer rows may have narrower chunks,
+  // at most 4 for each wide one, as long as those are below two an SM
   const size_t rows = (size_t)batch * beams;
-  const size_t chunks = (vocab + beam::CHUNK - 1) / beam::CHUNK;
-  const size_t most = 2 * (size_t)beam::BLOCKS * sms_or_default_count() + 2 * rows;
-  const size_t slots = rows * chunks < most ? rows * chunks : most;
-  return (slots * (topk + 1) * 8 + rows * 4 + 255) / 256 * 256;
+  const size_t wide = (vocab + beam::THREADS * 32 - 1) / (beam::THREADS * 32);
+  const size_t narrow = (vocab + beam::THREADS * 8 - 1) / (beam::THREADS * 8);
+  const size_t few = 8 * (size_t)sms_or_default_count() + 4 * wide;
+  const size_t low = rows * narrow < few ? rows * narrow : few;
+  const size_t slots = rows * wide > low ? rows * wide : low;
+  return (slots * (topk + 1) * 8 + 255) / 256 * 256;
 }
 
 int beam_topk_launch(const BeamArgs& a, cudaStream_t stream) {
@@ -570,17 +429,15 @@ int beam_topk_launch(const BeamArgs& a, cudaStream_t stream) {
   p.beams = a.beams;
   p.vocab = a.vocab;
   p.topk = a.topk;
-  beam::share(p);
-  const size_t rows = (size_t)a.batch * a.beams;
+  const uint32_t rows = a.batch * a.beams, per = beam::per_thread(rows, a.beams, a.vocab);
+  p.chunks = beam::chunks_of(rows, a.beams, a.vocab);
   p.keys = static_cast<beam::u64*>(a.workspace);
-  p.sums = reinterpret_cast<float2*>(p.keys + rows * p.parts * a.topk);
-  p.counts = reinterpret_cast<uint32_t*>(p.sums + rows * p.parts);
-  if (rows * p.parts * (a.topk + 1) * 8 + rows * 4 > beam_topk_workspace_bytes(a.batch, a.beams, a.vocab, a.topk))
-    return PVLC_WORKSPACE_TOO_SMALL;
+  p.sums = reinterpret_cast<float2*>(p.keys + (size_t)rows * p.chunks * a.topk);
   p.out_score = a.out_score;
   p.out_beam = a.out_beam;
   p.out_token = a.out_token;
   cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.chunks, rows);
   cfg.blockDim = dim3(beam::THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -590,11 +447,12 @@ int beam_topk_launch(const BeamArgs& a, cudaStream_t stream) {
   cfg.numAttrs = 1;
   const bool vec = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 &&
                    a.ld % (a.half_logits ? 8 : 4) == 0;
-  const int st = a.half_logits ? (vec ? beam::launch_chunks<__half, true>(p, cfg)
-                                      : beam::launch_chunks<__half, false>(p, cfg))
-                               : (vec ? beam::launch_chunks<float, true>(p, cfg)
-                                      : beam::launch_chunks<float, false>(p, cfg));
-  if (st) return st;
+  const cudaError_t e =
+      a.half_logits ? (vec ? beam::launch_chunks<__half, true>(p, per, cfg)
+                           : beam::launch_chunks<__half, false>(p, per, cfg))
+                    : (vec ? beam::launch_chunks<float, true>(p, per, cfg)
+                           : beam::launch_chunks<float, false>(p, per, cfg));
+  if (e != cudaSuccess) return PVLC_CUDA_ERROR;
   cfg.gridDim = dim3(a.batch);
   return cudaLaunchKernelEx(&cfg, beam::beam_join_kernel, p) == cudaSuccess ? PVLC_OK
                                                                             : PVLC_CUDA_ERROR;
