@@ -39,7 +39,7 @@ int check_cache(const pvlc_kv8_cache* c) {
 }
 
 size_t page_scratch(uint32_t batch, uint32_t slots, uint32_t pages) {
-  const size_t fork = 4 + 4 * (size_t)batch + slots, compact = 4 + 2 * (size_t)pages;
+  const size_t fork = 4 + 6 * (size_t)batch + slots, compact = 4 + 2 * (size_t)pages;
   return 4 * (fork > compact ? fork : compact);
 }
 

@@ -56,14 +56,15 @@ struct PageParams {
   uint32_t batch;
 };
 
-// Every slot is idle (-1) or in range, and none is named twice.  `seen` is a
-// bitmap over the slots in shared memory.
-__device__ bool slots_valid(const PageParams& p, uint32_t* seen) {
+// Copies the slots to shared memory; whether each is idle (-1) or in range, and
+// none is named twice.  `seen` is a bitmap over the slots in shared memory.
+__device__ bool slots_valid(const PageParams& p, uint32_t* seen, int32_t* slot) {
   for (uint32_t i = threadIdx.x; i < (p.slots + 31) / 32; i += PLAN_THREADS) seen[i] = 0;
+  for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) slot[b] = p.slot[b];
   __syncthreads();
   int bad = 0;
   for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
-    const int32_t s = p.slot[b];
+    const int32_t s = slot[b];
     if (s == -1) continue;
     if (s < 0 || (uint32_t)s >= p.slots) {
       bad = 1;
@@ -85,15 +86,18 @@ struct GrowParams {
 };
 
 __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowParams g) {
-  extern __shared__ uint32_t seen[];
+  extern __shared__ uint32_t sm[];         // the slots, then a bitmap over all slots
   const PageParams& p = g.b;
-  int bad = slots_valid(p, seen) ? 0 : (int)kFlagSlot;
+  int32_t* slot = reinterpret_cast<int32_t*>(sm);
+  pdl_wait();
+  pdl_launch_dependents();
+  int bad = slots_valid(p, sm + p.batch, slot) ? 0 : (int)kFlagSlot;
   // sequences [b0, b1) are this thread's: ranks follow the sequence order
   const uint32_t per = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS;
   const uint32_t b0 = min(p.batch, threadIdx.x * per), b1 = min(p.batch, b0 + per);
   if (!bad) {
     for (uint32_t b = b0; b < b1; ++b) {
-      const int32_t s = p.slot[b];
+      const int32_t s = slot[b];
       if (s < 0) continue;
       const int64_t adv = g.advance ? g.advance[b] : g.advance_by;
       const int64_t ahead = g.ahead ? g.ahead[b] : g.ahead_by;
@@ -109,7 +113,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
   }
   uint32_t need = 0;
   for (uint32_t b = b0; b < b1; ++b) {
-    const int32_t s = p.slot[b];
+    const int32_t s = slot[b];
     if (s < 0) continue;
     const int32_t n = p.tokens[s] + (g.advance ? g.advance[b] : g.advance_by);
     p.tokens[s] = n;
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
   found = min(found, total);
   __syncthreads();                       // the list is complete
   for (uint32_t b = b0; b < b1; ++b) {
-    const int32_t s = p.slot[b];
+    const int32_t s = slot[b];
     if (s < 0) continue;
     const int32_t n = p.tokens[s];
     const int32_t end = (n + (g.ahead ? g.ahead[b] : g.ahead_by)) / PAGE;
@@ -165,133 +169,132 @@ struct ForkParams {
   const int32_t* parent;
   int32_t* slot_out;
   int32_t advance_by;
-  // scratch: free slots [slots]; touched slots and where each copies from (-1:
-  // it is only emptied) [2 batch]; how many
+  // scratch: free slots [slots]; touched slots, where each copies from (-1: it is only
+  // emptied) and its rows [2 batch]; how many are copies, how many there are
   int32_t* free_list;
   int32_t* dst;
   int32_t* src;
-  uint32_t* touched;
+  int32_t* rows;
+  uint32_t* counts;
   __half* tails;
   uint32_t layers, heads;
 };
 
-// Shared memory: slots' bitmaps "named by slot[]" and "kept", then the eldest
-// child of every sequence.
+// Shared memory: the slots, the parents, the eldest child of every sequence, and
+// bitmaps over all slots: "named by slot[]" and "kept".
 __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const ForkParams f) {
   extern __shared__ uint32_t sm[];
+  __shared__ uint32_t emptied;
   const PageParams& p = f.b;
-  const uint32_t words = (p.slots + 31) / 32;
-  uint32_t* named = sm;
+  const uint32_t words = (p.slots + 31) / 32, tid = threadIdx.x;
+  int32_t* slot = reinterpret_cast<int32_t*>(sm);
+  int32_t* parent = slot + p.batch;
+  uint32_t* eldest = sm + 2 * p.batch;
+  uint32_t* named = eldest + p.batch;
   uint32_t* kept = named + words;
-  uint32_t* eldest = kept + words;
-  int bad = slots_valid(p, named) ? 0 : (int)kFlagSlot;
-  for (uint32_t i = threadIdx.x; i < words; i += PLAN_THREADS) kept[i] = 0;
-  for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
+  pdl_wait();
+  pdl_launch_dependents();
+  int bad = 0;
+  for (uint32_t i = tid; i < words; i += PLAN_THREADS) kept[i] = 0;
+  for (uint32_t b = tid; b < p.batch; b += PLAN_THREADS) {
     eldest[b] = 0xffffffffu;
-    const int32_t m = f.parent[b];
-    if (m < -1 || m >= (int32_t)p.batch) bad |= kFlagSlot;
+    parent[b] = f.parent[b];
+    if (parent[b] < -1 || parent[b] >= (int32_t)p.batch) bad |= kFlagSlot;
   }
+  if (tid == 0) emptied = 0;
+  if (!slots_valid(p, named, slot)) bad |= kFlagSlot;
   if (!bad)
-    for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
-      const int32_t s = p.slot[b];
-      if (s < 0) continue;
-      const int64_t n = p.tokens[s];
+    for (uint32_t b = tid; b < p.batch; b += PLAN_THREADS) {
+      if (slot[b] < 0) continue;
+      const int64_t n = p.tokens[slot[b]];
       if (n < 0 || !rows_fit(n + f.advance_by, p.max_pages)) bad |= kFlagCacheRow;
     }
-  const bool refuse = __syncthreads_or(bad);
-  if (threadIdx.x == 0) *f.touched = 0;
-  if (refuse) {                          // nothing is changed
+  if (__syncthreads_or(bad)) {           // nothing is changed
+    if (tid == 0) f.counts[0] = f.counts[1] = 0;
     if (bad) atomicOr(p.flags, (uint32_t)bad);
-    for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) f.slot_out[b] = p.slot[b];
+    for (uint32_t b = tid; b < p.batch; b += PLAN_THREADS) f.slot_out[b] = slot[b];
     return;
   }
-  for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
-    const int32_t s = p.slot[b];
-    if (s >= 0) p.tokens[s] += f.advance_by;
-    const int32_t m = f.parent[b];
-    if (m >= 0 && p.slot[m] >= 0) {
-      atomicMin(eldest + m, b);
-      atomicOr(kept + (p.slot[m] >> 5), 1u << (p.slot[m] & 31));
+  auto source = [&](uint32_t b) { return parent[b] >= 0 ? slot[parent[b]] : -1; };
+  for (uint32_t b = tid; b < p.batch; b += PLAN_THREADS) {
+    if (f.advance_by && slot[b] >= 0) p.tokens[slot[b]] += f.advance_by;
+    const int32_t s = source(b);
+    if (s >= 0) {
+      atomicMin(eldest + parent[b], b);
+      atomicOr(kept + (s >> 5), 1u << (s & 31));
     }
   }
   __syncthreads();
-  // free slots in ascending order: those given up here, and the empty ones
-  // that no sequence of this call names
+  // Free slots in ascending order: those given up here, and the empty ones that no
+  // sequence of this call names.  The children that need one, in sequence order.  One
+  // prefix sum for both: at most 65,536 slots below, at most 2,048 children above.
+  static_assert(PVLC_KV8_MAX_SLOTS <= 1u << 16 && PVLC_KV8_MAX_BATCH < 1u << 15, "packed counts");
   const uint32_t sper = (p.slots + PLAN_THREADS - 1) / PLAN_THREADS;
-  const uint32_t s0 = min(p.slots, threadIdx.x * sper), s1 = min(p.slots, s0 + sper);
+  const uint32_t s0 = min(p.slots, tid * sper), s1 = min(p.slots, s0 + sper);
   auto is_free = [&](uint32_t s) {
     const uint32_t bit = 1u << (s & 31);
     if (kept[s >> 5] & bit) return false;
     return (named[s >> 5] & bit) != 0 || p.tokens[s] == 0;
   };
-  uint32_t nfree = 0;
-  for (uint32_t s = s0; s < s1; ++s) nfree += is_free(s);
-  uint32_t free_total;
-  uint32_t r = block_scan(nfree, &free_total);
-  for (uint32_t s = s0; s < s1; ++s)
-    if (is_free(s)) f.free_list[r++] = s;
-  // the children that need a slot, in sequence order
   const uint32_t per = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS;
-  const uint32_t b0 = min(p.batch, threadIdx.x * per), b1 = min(p.batch, b0 + per);
-  auto moves = [&](uint32_t b) {
-    const int32_t m = f.parent[b];
-    return m >= 0 && p.slot[m] >= 0 && eldest[m] != b;
-  };
-  uint32_t n = 0;
-  for (uint32_t b = b0; b < b1; ++b) n += moves(b);
-  uint32_t children;
-  uint32_t rank = block_scan(n, &children);    // its barriers also publish free_list
+  const uint32_t b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+  auto moves = [&](uint32_t b) { return source(b) >= 0 && eldest[parent[b]] != b; };
+  uint32_t mine = 0;
+  for (uint32_t s = s0; s < s1; ++s) mine += is_free(s);
+  for (uint32_t b = b0; b < b1; ++b) mine += (uint32_t)moves(b) << 17;
+  uint32_t total;
+  const uint32_t before = block_scan(mine, &total);
+  const uint32_t free_total = total & 0x1ffff, children = total >> 17;
   const uint32_t given = min(children, free_total);
+  uint32_t r = before & 0x1ffff;
+  for (uint32_t s = s0; s < s1; ++s)
+    if (is_free(s)) {
+      f.free_list[r] = s;
+      if (r >= given && (named[s >> 5] >> (s & 31) & 1u)) {     // given up and not taken
+        const uint32_t e = given + atomicAdd(&emptied, 1);
+        f.dst[e] = s;
+        f.src[e] = -1;
+        f.rows[e] = 0;
+      }
+      ++r;
+    }
+  __syncthreads();                       // the list is complete
+  uint32_t rank = before >> 17;
   for (uint32_t b = b0; b < b1; ++b) {
-    const int32_t m = f.parent[b];
-    int32_t to = -1;
+    int32_t to = source(b);
     if (moves(b)) {
+      const int32_t from = to;
+      to = -1;
       if (rank < given) {
         to = f.free_list[rank];
         f.dst[rank] = to;
-        f.src[rank] = p.slot[m];
+        f.src[rank] = from;
+        f.rows[rank] = p.tokens[from];
       }
       ++rank;
-    } else if (m >= 0 && p.slot[m] >= 0) {
-      to = p.slot[m];
     }
     f.slot_out[b] = to;
   }
-  // slots given up and not taken: emptied
-  uint32_t emptied = 0;
-  auto empties = [&](uint32_t q) {      // rank q of the free list
-    const uint32_t s = f.free_list[q];
-    return (named[s >> 5] >> (s & 31) & 1u) != 0;
-  };
-  const uint32_t left = free_total - given;
-  const uint32_t fper = (left + PLAN_THREADS - 1) / PLAN_THREADS;
-  const uint32_t f0 = given + min(left, threadIdx.x * fper), f1 = min(free_total, f0 + fper);
-  for (uint32_t q = f0; q < f1; ++q) emptied += empties(q);
-  uint32_t emptied_total;
-  uint32_t e = given + block_scan(emptied, &emptied_total);
-  for (uint32_t q = f0; q < f1; ++q)
-    if (empties(q)) {
-      f.dst[e] = f.free_list[q];
-      f.src[e++] = -1;
-    }
-  if (threadIdx.x == 0) {
-    *f.touched = given + emptied_total;
+  if (tid == 0) {
+    f.counts[0] = given;
+    f.counts[1] = given + emptied;
     if (given < children) atomicOr(p.flags, kFlagExhausted);
   }
 }
 
-// Block (i, 0): the table row, count and page references of touched slot i;
-// block (i, 1 + l): its tail rows in layer l.  A source slot is a kept one and
-// a destination is not, so no block reads what another writes.
-__global__ void __launch_bounds__(128) kv8_fork_copy_kernel(const ForkParams f) {
+// A warp copies the open rows of one (copy, layer, K or V, head); a block does the
+// table row, count and page references of one touched slot.  A source slot is a
+// kept one and a destination is not, so nothing is read that another one writes.
+__global__ void __launch_bounds__(COPY_THREADS) kv8_fork_copy_kernel(const ForkParams f) {
   const PageParams& p = f.b;
-  if (blockIdx.x >= *f.touched) return;
-  const int32_t dst = f.dst[blockIdx.x], src = f.src[blockIdx.x];
-  const int32_t n = src >= 0 ? p.tokens[src] : 0;
-  if (blockIdx.y == 0) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t copies = f.counts[0], touched = f.counts[1];
+  for (uint32_t i = blockIdx.x; i < touched; i += gridDim.x) {
+    const int32_t dst = f.dst[i], src = f.src[i], n = f.rows[i];
     int32_t* to = p.table + (size_t)dst * p.max_pages;
     const int32_t* from = p.table + (size_t)(src >= 0 ? src : 0) * p.max_pages;
-    for (uint32_t j = threadIdx.x; j < p.max_pages; j += blockDim.x) {
+    for (uint32_t j = threadIdx.x; j < p.max_pages; j += COPY_THREADS) {
       const int32_t old = to[j];
       const int32_t page = (int32_t)j < n / PAGE ? from[j] : -1;
       if (old >= 0 && (uint32_t)old < p.pages) atomicSub(p.refs + old, 1);
@@ -299,17 +302,26 @@ __global__ void __launch_bounds__(128) kv8_fork_copy_kernel(const ForkParams f) 
       to[j] = page;
     }
     if (threadIdx.x == 0) p.tokens[dst] = n;
-    return;
   }
-  if (src < 0) return;
-  const uint32_t rows = n % PAGE;
-  const size_t layer = (size_t)(blockIdx.y - 1) * p.slots;
-  const uint4* from = reinterpret_cast<const uint4*>(f.tails + (layer + src) * 2 * f.heads * BLOCK_CODES);
-  uint4* to = reinterpret_cast<uint4*>(f.tails + (layer + dst) * 2 * f.heads * BLOCK_CODES);
-  const uint32_t per = rows * (HD / 8);        // 16-byte pieces of one (K/V, head)
-  for (uint32_t i = threadIdx.x; i < per * 2 * f.heads; i += blockDim.x) {
-    const size_t at = (size_t)(i / per) * (BLOCK_CODES / 8) + i % per;
-    to[at] = from[at];
+  const uint32_t lane = threadIdx.x & 31, parts = 2 * f.heads;
+  const uint32_t warp = blockIdx.x * (COPY_THREADS / 32) + (threadIdx.x >> 5);
+  const uint32_t warps = gridDim.x * (COPY_THREADS / 32), units = copies * f.layers * parts;
+  for (uint32_t u = warp; u < units; u += warps) {
+    const uint32_t i = u / (f.layers * parts), l = u / parts % f.layers, kvh = u % parts;
+    const int32_t dst = f.dst[i], src = f.src[i];
+    const uint32_t n = f.rows[i] % PAGE * (HD / 8);          // 16-byte pieces
+    const size_t layer = (size_t)l * p.slots;
+    const uint4* from = reinterpret_cast<const uint4*>(f.tails + ((layer + src) * parts + kvh) * BLOCK_CODES);
+    uint4* to = reinterpret_cast<uint4*>(f.tails + ((layer + dst) * parts + kvh) * BLOCK_CODES);
+    for (uint32_t e = lane; e < n; e += 4 * 32) {
+      uint4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + 32 * k < n) x[k] = from[e + 32 * k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + 32 * k < n) to[e + 32 * k] = x[k];
+    }
   }
 }
 
@@ -334,6 +346,8 @@ struct CompactParams {
 };
 
 __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_compact_plan_kernel(const CompactParams c) {
+  pdl_wait();
+  pdl_launch_dependents();
   uint32_t count = 0;
   for (uint32_t base = 0; base < c.a.pages; base += 4 * PLAN_THREADS) {
     const uint32_t at = base + 4 * threadIdx.x;
@@ -367,7 +381,22 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_compact_plan_kernel(const
   }
 }
 
+// n 16-byte pieces, four loads in flight a thread.
+__device__ __forceinline__ void copy_pieces(uint4* to, const uint4* from, uint32_t n) {
+  for (uint32_t e = threadIdx.x; e < n; e += 4 * COPY_THREADS) {
+    uint4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (e + k * COPY_THREADS < n) x[k] = __ldcs(from + e + k * COPY_THREADS);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (e + k * COPY_THREADS < n) __stcs(to + e + k * COPY_THREADS, x[k]);
+  }
+}
+
 __global__ void __launch_bounds__(COPY_THREADS) kv8_compact_copy_kernel(const CompactParams c) {
+  pdl_wait();
+  pdl_launch_dependents();
   const uint32_t live = *c.live;
   if (live == 0xffffffffu) return;       // nothing is changed
   const uint32_t t = blockIdx.x * COPY_THREADS + threadIdx.x, T = gridDim.x * COPY_THREADS;
@@ -387,9 +416,9 @@ __global__ void __launch_bounds__(COPY_THREADS) kv8_compact_copy_kernel(const Co
     const size_t from = (size_t)l * c.a.pages + c.order[i], to = (size_t)l * c.to_pages + i;
     for (uint32_t h = threadIdx.x; h < 2 * H; h += COPY_THREADS)
       c.to_scales[to * 2 * H + h] = c.scales[from * 2 * H + h];
-    const uint4* x = reinterpret_cast<const uint4*>(c.codes + from * 2 * H * BLOCK_CODES);
-    uint4* y = reinterpret_cast<uint4*>(c.to_codes + to * 2 * H * BLOCK_CODES);
-    for (uint32_t e = threadIdx.x; e < 2 * H * BLOCK_CODES / 16; e += COPY_THREADS) y[e] = x[e];
+    copy_pieces(reinterpret_cast<uint4*>(c.to_codes + to * 2 * H * BLOCK_CODES),
+                reinterpret_cast<const uint4*>(c.codes + from * 2 * H * BLOCK_CODES),
+                2 * H * BLOCK_CODES / 16);
   }
   // the open blocks' rows
   for (uint64_t u = blockIdx.x; u < (uint64_t)c.layers * c.a.slots; u += gridDim.x) {
@@ -420,6 +449,28 @@ PageParams page_params(const pvlc_kv8_cache& c, const int32_t* slot, uint32_t ba
 
 }  // namespace kv8
 
+namespace {
+
+// A launch that may start under the end of the kernel ahead of it; each of these
+// kernels waits for that one before it does anything.
+template <typename P>
+int launch(void (*kernel)(P), const P& params, dim3 grid, int threads, uint32_t smem,
+           cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, params) == cudaSuccess ? PVLC_OK : PVLC_CUDA_ERROR;
+}
+
+}  // namespace
+
 int kv8_grow_launch(const pvlc_kv8_cache& c, const int32_t* slot, uint32_t batch,
                     const int32_t* advance, int32_t advance_by, const int32_t* ahead,
                     int32_t ahead_by, void* ws, cudaStream_t stream) {
@@ -430,8 +481,8 @@ int kv8_grow_launch(const pvlc_kv8_cache& c, const int32_t* slot, uint32_t batch
   g.advance_by = advance_by;
   g.ahead_by = ahead_by;
   g.list = kv8_scratch(ws);
-  kv8::kv8_grow_kernel<<<1, kv8::PLAN_THREADS, (c.slots + 31) / 32 * 4, stream>>>(g);
-  return cudaPeekAtLastError() == cudaSuccess ? PVLC_OK : PVLC_CUDA_ERROR;
+  return launch(kv8::kv8_grow_kernel, g, dim3(1), kv8::PLAN_THREADS,
+                batch * 4 + (c.slots + 31) / 32 * 4, stream);
 }
 
 int kv8_fork_launch(const pvlc_kv8_cache& c, const int32_t* slot, const int32_t* parent,
@@ -442,18 +493,24 @@ int kv8_fork_launch(const pvlc_kv8_cache& c, const int32_t* slot, const int32_t*
   f.parent = parent;
   f.slot_out = slot_out;
   f.advance_by = advance_by;
+  const int sms = device_sm_count();
+  if (sms <= 0) return PVLC_CUDA_ERROR;
   int32_t* s = kv8_scratch(ws);
-  f.touched = reinterpret_cast<uint32_t*>(s);
+  f.counts = reinterpret_cast<uint32_t*>(s);
   f.dst = s + 4;
   f.src = f.dst + 2 * batch;
-  f.free_list = f.src + 2 * batch;
+  f.rows = f.src + 2 * batch;
+  f.free_list = f.rows + 2 * batch;
   f.tails = reinterpret_cast<__half*>(c.tails);
   f.layers = c.layers;
   f.heads = c.kv_heads;
-  const uint32_t smem = 2 * ((c.slots + 31) / 32) * 4 + batch * 4;
-  kv8::kv8_fork_plan_kernel<<<1, kv8::PLAN_THREADS, smem, stream>>>(f);
-  kv8::kv8_fork_copy_kernel<<<dim3(2 * batch, 1 + c.layers), 128, 0, stream>>>(f);
-  return cudaPeekAtLastError() == cudaSuccess ? PVLC_OK : PVLC_CUDA_ERROR;
+  const uint32_t smem = 3 * batch * 4 + 2 * ((c.slots + 31) / 32) * 4;
+  if (const int st = launch(kv8::kv8_fork_plan_kernel, f, dim3(1), kv8::PLAN_THREADS, smem, stream))
+    return st;
+  // a warp for each copy where all but one sequence move, up to eight blocks an SM
+  const uint64_t blocks = ((uint64_t)batch * c.layers * 2 * c.kv_heads + 7) / 8;
+  return launch(kv8::kv8_fork_copy_kernel, f, dim3((uint32_t)(blocks < 8u * sms ? blocks : 8u * sms)),
+                kv8::COPY_THREADS, 0, stream);
 }
 
 int kv8_compact_launch(const pvlc_kv8_cache& a, const pvlc_kv8_cache& b, int32_t* live_out,
@@ -481,9 +538,9 @@ int kv8_compact_launch(const pvlc_kv8_cache& a, const pvlc_kv8_cache& b, int32_t
   c.order = s + 4;
   c.map = c.order + a.pages;
   c.live_out = live_out;
-  kv8::kv8_compact_plan_kernel<<<1, kv8::PLAN_THREADS, 0, stream>>>(c);
-  kv8::kv8_compact_copy_kernel<<<8 * sms, kv8::COPY_THREADS, 0, stream>>>(c);
-  return cudaPeekAtLastError() == cudaSuccess ? PVLC_OK : PVLC_CUDA_ERROR;
+  if (const int st = launch(kv8::kv8_compact_plan_kernel, c, dim3(1), kv8::PLAN_THREADS, 0, stream))
+    return st;
+  return launch(kv8::kv8_compact_copy_kernel, c, dim3(8 * sms), kv8::COPY_THREADS, 0, stream);
 }
 
 }  // namespace pvlc
