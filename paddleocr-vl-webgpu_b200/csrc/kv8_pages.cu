@@ -381,25 +381,69 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_compact_plan_kernel(const
   }
 }
 
-// n 16-byte pieces, four loads in flight a thread.
-__device__ __forceinline__ void copy_pieces(uint4* to, const uint4* from, uint32_t n) {
-  for (uint32_t e = threadIdx.x; e < n; e += 4 * COPY_THREADS) {
-    uint4 x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (e + k * COPY_THREADS < n) x[k] = __ldcs(from + e + k * COPY_THREADS);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (e + k * COPY_THREADS < n) __stcs(to + e + k * COPY_THREADS, x[k]);
-  }
-}
+// Pages move through shared memory in pieces of 8 KB (a head's share), each by one
+// bulk copy in and one out, so that no registers or load slots bound the bytes in
+// flight: two warps of 12 lanes, a stage each, 192 KB an SM.  The two warps' reads
+// and writes alternate against each other.  The other warps do the small things.
+constexpr uint32_t PIECE = 2 * BLOCK_CODES;
+constexpr uint32_t LANES = 12, ENGINES = 2;
+constexpr uint32_t COMPACT_SMEM = LANES * ENGINES * (PIECE + 8);
 
-__global__ void __launch_bounds__(COPY_THREADS) kv8_compact_copy_kernel(const CompactParams c) {
+__global__ void __launch_bounds__(COPY_THREADS, 1) kv8_compact_copy_kernel(const CompactParams c) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + LANES * ENGINES * PIECE);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < ENGINES && lane < LANES) {
+    mbar_init(bars + warp * LANES + lane, 1);
+    fence_mbar_init();
+  }
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t live = *c.live;
   if (live == 0xffffffffu) return;       // nothing is changed
-  const uint32_t t = blockIdx.x * COPY_THREADS + threadIdx.x, T = gridDim.x * COPY_THREADS;
+  const uint32_t H = c.heads;
+  if (warp < ENGINES) {
+    uint8_t* stage = ring + (warp * LANES + lane) * PIECE;
+    uint64_t* bar = bars + warp * LANES + lane;
+    const uint64_t n = (uint64_t)c.layers * live * H;
+    const uint64_t step = (uint64_t)gridDim.x * ENGINES * LANES;
+    uint32_t phase = 0;
+    __syncwarp();
+    for (uint64_t first = (uint64_t)(blockIdx.x * ENGINES + warp) * LANES; first < n; first += step) {
+      const uint64_t k = first + lane;
+      const bool on = lane < LANES && k < n;
+      size_t to = 0;
+      if (on) {
+        const uint64_t u = k / H;
+        const uint32_t l = (uint32_t)(u / live), i = (uint32_t)(u % live), part = (uint32_t)(k % H);
+        const size_t from = ((size_t)l * c.a.pages + c.order[i]) * H + part;
+        to = ((size_t)l * c.to_pages + i) * H + part;
+        // the stage's last copy out has been read
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        mbar_arrive_expect_tx(bar, PIECE);
+        bulk_g2s(stage, c.codes + from * PIECE, PIECE, bar);
+      }
+      const bool landed = !on || mbar_wait(bar, phase);
+      if (!__all_sync(0xffffffffu, landed)) {
+        if (lane == 0) atomicOr(c.a.flags, kFlagTimeout);
+        if (on) mbar_wait(bar, phase);   // leave no copy in flight
+        break;
+      }
+      phase ^= 1;
+      if (on) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                         c.to_codes + to * PIECE),
+                     "r"(smem_u32(stage)), "r"(PIECE)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    return;
+  }
+  constexpr uint32_t REST = COPY_THREADS - ENGINES * 32;
+  const uint32_t tid = threadIdx.x - ENGINES * 32;
+  const uint32_t t = blockIdx.x * REST + tid, T = gridDim.x * REST;
   // the tables, counts and references
   for (uint64_t i = t; i < (uint64_t)c.to_slots * c.to_max_pages; i += T) {
     const uint32_t s = (uint32_t)(i / c.to_max_pages), j = (uint32_t)(i % c.to_max_pages);
@@ -409,26 +453,30 @@ __global__ void __launch_bounds__(COPY_THREADS) kv8_compact_copy_kernel(const Co
   }
   for (uint32_t s = t; s < c.to_slots; s += T) c.to_tokens[s] = s < c.a.slots ? c.a.tokens[s] : 0;
   for (uint32_t i = t; i < c.to_pages; i += T) c.to_refs[i] = i < live ? c.a.refs[c.order[i]] : 0;
-  // scales, then codes: one block takes a (layer, page) at a time
-  const uint32_t H = c.heads;
-  for (uint64_t u = blockIdx.x; u < (uint64_t)c.layers * live; u += gridDim.x) {
-    const uint32_t l = (uint32_t)(u / live), i = (uint32_t)(u % live);
-    const size_t from = (size_t)l * c.a.pages + c.order[i], to = (size_t)l * c.to_pages + i;
-    for (uint32_t h = threadIdx.x; h < 2 * H; h += COPY_THREADS)
-      c.to_scales[to * 2 * H + h] = c.scales[from * 2 * H + h];
-    copy_pieces(reinterpret_cast<uint4*>(c.to_codes + to * 2 * H * BLOCK_CODES),
-                reinterpret_cast<const uint4*>(c.codes + from * 2 * H * BLOCK_CODES),
-                2 * H * BLOCK_CODES / 16);
+  // scales
+  for (uint64_t e = t; e < (uint64_t)c.layers * live * 2 * H; e += T) {
+    const uint64_t u = e / (2 * H);
+    const uint32_t l = (uint32_t)(u / live), i = (uint32_t)(u % live), h = (uint32_t)(e % (2 * H));
+    c.to_scales[((size_t)l * c.to_pages + i) * 2 * H + h] =
+        c.scales[((size_t)l * c.a.pages + c.order[i]) * 2 * H + h];
   }
-  // the open blocks' rows
-  for (uint64_t u = blockIdx.x; u < (uint64_t)c.layers * c.a.slots; u += gridDim.x) {
-    const uint32_t l = (uint32_t)(u / c.a.slots), s = (uint32_t)(u % c.a.slots);
-    const uint32_t per = c.a.tokens[s] % PAGE * (HD / 8);
-    const uint4* x = reinterpret_cast<const uint4*>(c.tails + ((size_t)l * c.a.slots + s) * 2 * H * BLOCK_CODES);
-    uint4* y = reinterpret_cast<uint4*>(c.to_tails + ((size_t)l * c.to_slots + s) * 2 * H * BLOCK_CODES);
-    for (uint32_t e = threadIdx.x; e < per * 2 * H; e += COPY_THREADS) {
-      const size_t at = (size_t)(e / per) * (BLOCK_CODES / 8) + e % per;
-      y[at] = x[at];
+  // the open blocks' rows: a warp takes one (layer, slot, K or V, head)
+  const uint32_t parts = 2 * H, warps = T / 32;
+  for (uint64_t u = t / 32; u < (uint64_t)c.layers * c.a.slots * parts; u += warps) {
+    const uint32_t l = (uint32_t)(u / parts / c.a.slots), s = (uint32_t)(u / parts % c.a.slots);
+    const uint32_t kvh = (uint32_t)(u % parts), n = c.a.tokens[s] % PAGE * (HD / 8);
+    const uint4* x = reinterpret_cast<const uint4*>(
+        c.tails + (((size_t)l * c.a.slots + s) * parts + kvh) * BLOCK_CODES);
+    uint4* y = reinterpret_cast<uint4*>(
+        c.to_tails + (((size_t)l * c.to_slots + s) * parts + kvh) * BLOCK_CODES);
+    for (uint32_t e = lane; e < n; e += 4 * 32) {
+      uint4 z[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + 32 * k < n) z[k] = x[e + 32 * k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + 32 * k < n) y[e + 32 * k] = z[k];
     }
   }
 }
@@ -540,7 +588,11 @@ int kv8_compact_launch(const pvlc_kv8_cache& a, const pvlc_kv8_cache& b, int32_t
   c.live_out = live_out;
   if (const int st = launch(kv8::kv8_compact_plan_kernel, c, dim3(1), kv8::PLAN_THREADS, 0, stream))
     return st;
-  return launch(kv8::kv8_compact_copy_kernel, c, dim3(8 * sms), kv8::COPY_THREADS, 0, stream);
+  if (const int st = set_smem_attribute_once(
+          reinterpret_cast<const void*>(kv8::kv8_compact_copy_kernel), kv8::COMPACT_SMEM))
+    return st;
+  return launch(kv8::kv8_compact_copy_kernel, c, dim3(sms), kv8::COPY_THREADS, kv8::COMPACT_SMEM,
+                stream);
 }
 
 }  // namespace pvlc
