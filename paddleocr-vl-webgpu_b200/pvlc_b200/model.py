@@ -186,6 +186,7 @@ class OcrEngine:
         self.lm_head = dw[2 + 9 * c.decoder_layers]
         self._grid_cache = {}
         self._decode = None
+        self._beam = None
 
     @classmethod
     def from_checkpoint(cls, path, cfg: ModelConfig | None = None, device=None, **kw):
@@ -339,8 +340,53 @@ class OcrEngine:
     def _logits(self, fn):
         return torch.mm(fn, self.lm_head.t(), out_dtype=torch.float32)
 
+    def _plan_prompts(self, grids) -> "_PromptPlan":
+        """The host's share of a prefill: prompt ids, packed offsets, M-RoPE tables, and one
+        pinned, asynchronous upload of the indices."""
+        c = self.cfg
+        B = len(grids)
+        m2 = c.merge * c.merge
+        ids = [ocr_prompt_ids(g[0] * g[1] * g[2] // m2, c) for g in grids]
+        Ts = [len(x) for x in ids]
+        offs = np.concatenate([[0], np.cumsum(Ts)]).astype(np.int64)
+        flat = np.concatenate([np.asarray(x, dtype=np.int64) for x in ids])
+        img_pos = np.flatnonzero(flat == c.image_token_id)
+        if img_pos.size != sum(g[0] * g[1] * g[2] // m2 for g in grids):
+            raise ValueError("image placeholder count does not match the images")
+        tables, deltas = [], []
+        for x, g in zip(ids, grids):
+            tc, ts, delta = self._prompt_tables(x, g)
+            tables.append((tc, ts))
+            deltas.append(delta)
+        plan = _upload(np.concatenate([flat, img_pos, offs[1:] - 1]), self.device)
+        ids_t, img_idx, last = torch.split(plan, [int(offs[-1]), int(img_pos.size), B])
+        return _PromptPlan(Ts, offs, tables, deltas, ids_t, img_idx, last)
+
+    def _prefill(self, plan: "_PromptPlan", img, caches, stored=None):
+        """Prefill of all prompts: GEMMs over all rows, attention per prompt.  caches(l): layer
+        l's [B, capacity, 2, 128] fp16 K and V caches; stored(l), when given, is called once
+        they are written.  Returns the final norm of every row."""
+        c, dev = self.cfg, self.device
+        NT = int(plan.offsets[-1])
+        QW = c.query_heads * c.head_dim
+        emb = self.embed.index_select(0, plan.ids)
+        emb.index_copy_(0, plan.image_rows, torch.cat(img, 0))
+        h32 = emb.float()
+        ctx = torch.empty((NT, c.query_heads, c.head_dim), dtype=torch.float16, device=dev)
+        pending = None
+        for l, L in enumerate(self.dlayers):
+            n1 = ops.add_norm(h32, L["n1"], c.rms_eps, delta=pending)
+            q = F.linear(n1, L["q"]).view(NT, c.query_heads, c.head_dim)
+            k = F.linear(n1, L["k"]).view(NT, c.kv_heads, c.head_dim)
+            v = F.linear(n1, L["v"]).view(NT, c.kv_heads, c.head_dim)
+            ops.decoder_prefill_packed(q, k, v, plan.offsets, plan.tables, *caches(l), ctx)
+            if stored is not None:
+                stored(l)
+            pending = self._layer_mlp(L, h32, F.linear(ctx.view(NT, QW), L["o"]))
+        return ops.add_norm(h32, self.final_norm, c.rms_eps, delta=pending)
+
     def recognize(self, images, max_new_tokens: int = 512, chunk: int = 32,
-                  preprocess_config=None, timings: dict | None = None):
+                  preprocess_config=None, timings: dict | None = None, beams: int = 1, **search):
         """Greedy OCR of host RGB8 pages ([H, W, 3] uint8 numpy arrays or CPU tensors).
 
         Each page is copied to the device (pinned staging), resized and cut into patches
@@ -348,7 +394,8 @@ class OcrEngine:
         runs the model.  All pages share one device buffer and all patches another, in
         page order, so the call makes two allocations whatever the page count and the
         encoder reads each vision batch's patches in place; each vision batch's pages are
-        uploaded and cut just before that batch is encoded.  Returns generate()'s dict."""
+        uploaded and cut just before that batch is encoded.  Returns generate()'s dict, or
+        with beams > 1 (and generate_beam's other options) generate_beam()'s."""
         from . import preprocess
         cfgp = preprocess_config or preprocess.MODEL_CONFIG
         ps = cfgp.patch_size
@@ -382,8 +429,24 @@ class OcrEngine:
                 d.copy_(t, non_blocking=True)
                 ops.image_patches(d, h, w, ps, out=out, workspace=ws)
 
+        if beams > 1 or search:
+            return self.generate_beam(patches, grids, max_new_tokens, beams=beams, chunk=chunk,
+                                      timings=timings, prepare=prepare, **search)
         return self.generate(patches, grids, max_new_tokens, chunk=chunk, timings=timings,
                              prepare=prepare)
+
+    def generate_beam(self, images_patches, grids, max_new_tokens: int, beams: int = 4,
+                      length_penalty: float = 1.0, cache_dtype=torch.float8_e4m3fn,
+                      chunk: int = 16, timings: dict | None = None, prepare=None,
+                      record: bool = False):
+        """Beam-searched OCR of B requests over an 8-bit paged KV cache (pvlc_b200.beam):
+        generate()'s inputs; returns dict(tokens=the best hypothesis of each request,
+        stop=its reason, hypotheses=per request the list of (score, tokens, reason), best
+        first).  A hypothesis scores its log-probability over its length to the power
+        length_penalty.  cache_dtype: float8_e4m3fn or int8."""
+        from . import beam
+        return beam.generate(self, images_patches, grids, max_new_tokens, beams, length_penalty,
+                             cache_dtype, chunk, timings, prepare, record)
 
     def generate(self, images_patches, grids, max_new_tokens: int, chunk: int = 16,
                  record_logits: bool = False, timings: dict | None = None, prepare=None):
@@ -398,54 +461,26 @@ class OcrEngine:
         device except the reads of the first tokens and of each chunk's tokens: the
         prompt plan is built and uploaded (pinned, asynchronous) before the encoder is
         queued, and the next decode chunk is queued before a chunk's tokens are read."""
-        c, dev = self.cfg, self.device
+        c = self.cfg
         B = len(grids)
-        m2 = c.merge * c.merge
         ev = None
         if timings is not None:
             ev = [torch.cuda.Event(enable_timing=True) for _ in range(5)]
             ev[4].record()
         # ---- host-side prompt plan
-        ids = [ocr_prompt_ids(g[0] * g[1] * g[2] // m2, c) for g in grids]
-        Ts = [len(x) for x in ids]
+        plan = self._plan_prompts(grids)
+        Ts = plan.lengths
         cap = max(Ts) + max_new_tokens + 1
-        offs = np.concatenate([[0], np.cumsum(Ts)]).astype(np.int64)
-        NT = int(offs[-1])
-        flat = np.concatenate([np.asarray(x, dtype=np.int64) for x in ids])
-        img_pos = np.flatnonzero(flat == c.image_token_id)
-        if img_pos.size != sum(g[0] * g[1] * g[2] // m2 for g in grids):
-            raise ValueError("image placeholder count does not match the images")
-        tables, deltas = [], []
-        for x, g in zip(ids, grids):
-            tc, ts, delta = self._prompt_tables(x, g)
-            tables.append((tc, ts))
-            deltas.append(delta)
-        plan = _upload(np.concatenate([flat, img_pos, offs[1:] - 1]), dev)
-        ids_t, img_idx, last = torch.split(plan, [NT, int(img_pos.size), B])
+        last = plan.last
         if ev:
             ev[0].record()
         img = self.encode_images(images_patches, grids, prepare)
         if ev:
             ev[1].record()
-        QW = c.query_heads * c.head_dim
         # the KV caches and the decode step's graph belong to the batch shape (B, cap) and
         # are reused by the next call of the same shape
         dec = self._decode_buffers(B, cap)
-        kc, vc = dec.kc, dec.vc
-        # ---- prefill: GEMMs over all prompts, attention per prompt
-        emb = self.embed.index_select(0, ids_t)
-        emb.index_copy_(0, img_idx, torch.cat(img, 0))
-        h32 = emb.float()
-        ctx = torch.empty((NT, c.query_heads, c.head_dim), dtype=torch.float16, device=dev)
-        pending = None
-        for l, L in enumerate(self.dlayers):
-            n1 = ops.add_norm(h32, L["n1"], c.rms_eps, delta=pending)
-            q = F.linear(n1, L["q"]).view(NT, c.query_heads, c.head_dim)
-            k = F.linear(n1, L["k"]).view(NT, c.kv_heads, c.head_dim)
-            v = F.linear(n1, L["v"]).view(NT, c.kv_heads, c.head_dim)
-            ops.decoder_prefill_packed(q, k, v, offs, tables, kc[l], vc[l], ctx)
-            pending = self._layer_mlp(L, h32, F.linear(ctx.view(NT, QW), L["o"]))
-        fn = ops.add_norm(h32, self.final_norm, c.rms_eps, delta=pending)
+        fn = self._prefill(plan, img, lambda l: (dec.kc[l], dec.vc[l]))
         if record_logits:
             logits0 = self._logits(fn.index_select(0, last))
             first = torch.argmax(logits0, dim=-1)
@@ -457,7 +492,7 @@ class OcrEngine:
         rec = [_download(logits0)] if record_logits else None
         # ---- batched decode, one CUDA graph per step shape; one chunk always queued
         # ahead of the chunk whose tokens are being applied
-        dec.reset(first, np.asarray(Ts), np.asarray(deltas))
+        dec.reset(first, np.asarray(Ts), np.asarray(plan.deltas))
         inflight = []
         budget = max_new_tokens - 1        # decode steps a request can still need
 
@@ -497,6 +532,18 @@ class OcrEngine:
             allg = torch.cat([r.unsqueeze(0) if r.dim() == 2 else r for r in rec], 0)  # [S,B,V]
             out["logits"] = [allg[: state.count[b], b] for b in range(B)]
         return out
+
+
+@dataclass
+class _PromptPlan:
+    """One batch's prompts, packed back to back."""
+    lengths: list          # rows of each prompt
+    offsets: np.ndarray    # [B + 1] their first rows
+    tables: list           # M-RoPE (cos, sin) of each prompt (device)
+    deltas: list           # position of a decode row minus its cache row
+    ids: torch.Tensor      # [rows] token ids (device)
+    image_rows: torch.Tensor
+    last: torch.Tensor     # [B] each prompt's last row
 
 
 def _join_rows(ts):
