@@ -24,6 +24,9 @@
 //     ahead in the table.  A page's scales follow by cp.async on the same barrier.
 //   * Four consumer warps take the pages in turn, each with its own running
 //     (O, M, L), so they meet only at a unit's end.
+//   * The rotated q goes in as its fp16 rounding and the rest of it, two operands,
+//     so the scores are exact to f32; the weights' fp16 rounding (2^-11 each, many
+//     of them averaged) is the one loss before the output's own.
 //   * S^T = K Q^T and O^T += V^T W^T with mma.m16n8k16: the 8 query heads of a
 //     group are the N side (two N tiles above 8).  The contraction order is
 //     free, so a lane's 16-byte loads are whole operand fragments: 16 dims of a
@@ -89,10 +92,19 @@ __device__ __forceinline__ uint32_t check_sequence(const DecodeParams& p, uint32
   return bad;
 }
 
+// Two values as an fp16 pair, and what that rounds off as another.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& pair, uint32_t& rest) {
+  pair = pack_half2(a, b);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+  rest = pack_half2(a - h.x, b - h.y);
+}
+
 // 16 dims d .. d + 15 (d a multiple of 16, below 64) and their partners 64
-// above, rotated: lo cos - hi sin, hi cos + lo sin; as fp16 pairs.
+// above, rotated: lo cos - hi sin, hi cos + lo sin; as fp16 pairs, and what those
+// round off.
 __device__ __forceinline__ void rotate16(const __half* row, uint32_t d, const DecodeParams& p,
-                                         uint32_t r, uint32_t* lo_out, uint32_t* hi_out) {
+                                         uint32_t r, uint32_t* lo_out, uint32_t* hi_out,
+                                         uint32_t* lo_rest, uint32_t* hi_rest) {
 #pragma unroll
   for (int e = 0; e < 16; e += 4) {
     const uint2 lw = __ldg(reinterpret_cast<const uint2*>(row + d + e));
@@ -109,10 +121,13 @@ __device__ __forceinline__ void rotate16(const __half* row, uint32_t d, const De
     auto turn = [](float x, float c, float y, float s) {
       return __fadd_rn(__fmul_rn(x, c), __fmul_rn(y, s));
     };
-    lo_out[e / 2] = pack_half2(turn(l0.x, cl.x, -h0.x, sl.x), turn(l0.y, cl.y, -h0.y, sl.y));
-    lo_out[e / 2 + 1] = pack_half2(turn(l1.x, cl.z, -h1.x, sl.z), turn(l1.y, cl.w, -h1.y, sl.w));
-    hi_out[e / 2] = pack_half2(turn(h0.x, ch.x, l0.x, sh.x), turn(h0.y, ch.y, l0.y, sh.y));
-    hi_out[e / 2 + 1] = pack_half2(turn(h1.x, ch.z, l1.x, sh.z), turn(h1.y, ch.w, l1.y, sh.w));
+    const int w = e / 2;
+    split2(turn(l0.x, cl.x, -h0.x, sl.x), turn(l0.y, cl.y, -h0.y, sl.y), lo_out[w], lo_rest[w]);
+    split2(turn(l1.x, cl.z, -h1.x, sl.z), turn(l1.y, cl.w, -h1.y, sl.w), lo_out[w + 1],
+           lo_rest[w + 1]);
+    split2(turn(h0.x, ch.x, l0.x, sh.x), turn(h0.y, ch.y, l0.y, sh.y), hi_out[w], hi_rest[w]);
+    split2(turn(h1.x, ch.z, l1.x, sh.z), turn(h1.y, ch.w, l1.y, sh.w), hi_out[w + 1],
+           hi_rest[w + 1]);
   }
 }
 
@@ -207,35 +222,62 @@ __device__ __forceinline__ void weigh(float (&s)[2][NT][4], Acc<NT>& a, float kk
   }
 }
 
+// The lane's fragments of q's rounding rest, words 4 i .. 4 i + 3 of N tile nt.
+__device__ __forceinline__ uint4 rest_words(const uint8_t* rest, int nt, int i) {
+  return reinterpret_cast<const uint4*>(rest)[(nt * 4 + i) * 32 + (threadIdx.x & 31)];
+}
+
 // One page of codes at `st` (K, then V 4 KB above, both swizzled).
 template <int CODE, int NT>
 __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv, float qk,
-                                          const uint32_t (&qf)[NT][16], Acc<NT>& a, int g, int t) {
+                                          const uint32_t (&qf)[NT][16], const uint8_t* rest,
+                                          Acc<NT>& a, int g, int t) {
   const int pi = (g >> 1) | ((g & 1) << 2);
-  float s[2][NT][4];
+  float s[2][NT][4], low[2][NT][4];
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt) {
+  for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[mt][nt][e] = low[mt][nt][e] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < 2; ++j) {
+    uint32_t wa[2][4], wb[2][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
       const uint8_t* at = st + (16 * mt + pi) * HD + (((t + 4 * j) ^ pi) << 4);
       const uint4 xa = *reinterpret_cast<const uint4*>(at);
       const uint4 xb = *reinterpret_cast<const uint4*>(at + 8 * HD);
-      const uint32_t wa[4] = {xa.x, xa.y, xa.z, xa.w}, wb[4] = {xb.x, xb.y, xb.z, xb.w};
+      wa[mt][0] = xa.x, wa[mt][1] = xa.y, wa[mt][2] = xa.z, wa[mt][3] = xa.w;
+      wb[mt][0] = xb.x, wb[mt][1] = xb.y, wb[mt][2] = xb.z, wb[mt][3] = xb.w;
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t ya = biased<CODE>(wa[e]), yb = biased<CODE>(wb[e]);
-        const uint32_t a0 = codes_lo<CODE>(ya), a1 = codes_lo<CODE>(yb);
-        const uint32_t a2 = codes_hi<CODE>(ya), a3 = codes_hi<CODE>(yb);
+    for (int f = 0; f < 2; ++f) {
+      uint4 r[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma_16816(s[mt][nt], a0, a1, a2, a3, qf[nt][8 * j + 2 * e], qf[nt][8 * j + 2 * e + 1]);
-      }
+      for (int nt = 0; nt < NT; ++nt) r[nt] = rest_words(rest, nt, 2 * j + f);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const int i = 2 * f + e;
+          const uint32_t ya = biased<CODE>(wa[mt][i]), yb = biased<CODE>(wb[mt][i]);
+          const uint32_t a0 = codes_lo<CODE>(ya), a1 = codes_lo<CODE>(yb);
+          const uint32_t a2 = codes_hi<CODE>(ya), a3 = codes_hi<CODE>(yb);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_16816(s[mt][nt], a0, a1, a2, a3, qf[nt][8 * j + 2 * i], qf[nt][8 * j + 2 * i + 1]);
+            mma_16816(low[mt][nt], a0, a1, a2, a3, e ? r[nt].z : r[nt].x, e ? r[nt].w : r[nt].y);
+          }
+        }
     }
   }
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[mt][nt][e] += low[mt][nt][e];
   uint32_t w[2][NT][2];
   weigh<NT>(s, a, sk * qk, __log2f(sv), __frcp_rn(sv), 0, 64, w);
   // value rows t, t + 4, t + 8, t + 12 of a half tile: keys pi(2 t), pi(2 t + 1), ..
@@ -270,7 +312,8 @@ __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv,
 template <int NT>
 __device__ __forceinline__ void tail_tile(const uint8_t* kt, const uint8_t* vt, const uint8_t* kn,
                                           const uint8_t* vn, int last, float qk,
-                                          const uint32_t (&qf)[NT][16], Acc<NT>& a, int g, int t) {
+                                          const uint32_t (&qf)[NT][16], const uint8_t* rest,
+                                          Acc<NT>& a, int g, int t) {
   const int pi = (g >> 1) | ((g & 1) << 2);
   float s[2][NT][4];
 #pragma unroll
@@ -291,8 +334,11 @@ __device__ __forceinline__ void tail_tile(const uint8_t* kt, const uint8_t* vt, 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const uint32_t* qq = qf[nt] + 8 * j + 4 * f;
+          const uint4 r = rest_words(rest, nt, 2 * j + f);
           mma_16816(s[mt][nt], xa.x, xb.x, xa.y, xb.y, qq[0], qq[1]);
+          mma_16816(s[mt][nt], xa.x, xb.x, xa.y, xb.y, r.x, r.y);
           mma_16816(s[mt][nt], xa.z, xb.z, xa.w, xb.w, qq[2], qq[3]);
+          mma_16816(s[mt][nt], xa.z, xb.z, xa.w, xb.w, r.z, r.w);
         }
       }
   }
@@ -481,10 +527,10 @@ struct Units {
   }
 };
 
-// A unit's rotated q as the consumers' fragments [NT][4][32 lanes] x 16 bytes, then its new
-// key and value rows.
+// A unit's rotated q as the consumers' fragments [NT][4][32 lanes] x 16 bytes, what it rounds
+// off in the same form, then its new key and value rows.
 template <int NT>
-constexpr uint32_t seq_slot() { return NT * 2048 + 512; }
+constexpr uint32_t seq_slot() { return 2 * NT * 2048 + 512; }
 
 template <int NT>
 constexpr uint32_t fixed_smem() {
@@ -691,29 +737,31 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       uint8_t* slot = slots + s * seq_slot<NT>();
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        uint32_t w[16];
+        uint32_t w[16], rest[16];
         const uint32_t head = nt * 8 + (lane >> 2);
         if (head < G) {
           rotate16(p.q + (size_t)it.b * p.q_stride + ((size_t)it.h * G + head) * HD,
-                   16 * (lane & 3), p, it.sq.rope, w, w + 8);
+                   16 * (lane & 3), p, it.sq.rope, w, w + 8, rest, rest + 8);
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = 0;
+          for (int e = 0; e < 16; ++e) w[e] = rest[e] = 0;
         }
+        uint4* to = reinterpret_cast<uint4*>(slot) + nt * 128 + lane;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          reinterpret_cast<uint4*>(slot)[(nt * 4 + e) * 32 + lane] =
-              make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        for (int e = 0; e < 4; ++e) {
+          to[e * 32] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          to[NT * 128 + e * 32] = make_uint4(rest[4 * e], rest[4 * e + 1], rest[4 * e + 2], rest[4 * e + 3]);
+        }
       }
       mbar_arrive(q_full + s);
       if (it.has_tail()) {
         const int last = it.sq.rows % PAGE;
-        uint4* kn = reinterpret_cast<uint4*>(slot + NT * 2048);
+        uint4* kn = reinterpret_cast<uint4*>(slot + 2 * NT * 2048);
         uint4* vn = kn + 16;
         if (lane < 4) {
-          uint32_t w[16];
+          uint32_t w[16], rest[16];
           rotate16(p.k_new + (size_t)it.b * p.kv_stride + it.h * HD, 16 * lane, p, it.sq.rope, w,
-                   w + 8);
+                   w + 8, rest, rest + 8);
           uint4* row = reinterpret_cast<uint4*>(tail_rows(p.c, it.sq.slot, 0, it.h) + last * HD);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -837,7 +885,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           // --------------------------------------------------------- tail
           seek(at);
           const int last = sq.rows % PAGE;
-          const uint8_t* rows = slot + NT * 2048;
+          const uint8_t* rows = slot + 2 * NT * 2048;
           const uint32_t s0 = stage;
           landed();
           const uint8_t* kt = ring + stage * STAGE;
@@ -845,7 +893,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           landed();
           const uint8_t* vt = ring + stage * STAGE;
           if (arrived(row_full + (unit & 1), slot_phase)) {
-            tail_tile<NT>(kt, vt, rows, rows + 256, last, qk, qf, a, g, t);
+            tail_tile<NT>(kt, vt, rows, rows + 256, last, qk, qf, slot + NT * 2048, a, g, t);
           }
           release(stage);
           release(s0);
@@ -856,7 +904,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           seek(at + i - i0 + skew);
           if (landed()) {
             const float2 sc = scale[stage];
-            page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, a, g, t);
+            page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, slot + NT * 2048, a, g, t);
           }
           release(stage);
         }
