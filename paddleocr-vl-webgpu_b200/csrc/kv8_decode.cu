@@ -92,19 +92,25 @@ __device__ __forceinline__ uint32_t check_sequence(const DecodeParams& p, uint32
   return bad;
 }
 
-// Two values as an fp16 pair, and what that rounds off as another.
+// Two values as an fp16 pair, and what that rounds off (or cuts off, beyond
+// fp16's range) as another.
+__device__ __forceinline__ float in_range(float x) {      // a NaN stays one
+  return x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
+}
 __device__ __forceinline__ void split2(float a, float b, uint32_t& pair, uint32_t& rest) {
-  pair = pack_half2(a, b);
+  pair = pack_half2(in_range(a), in_range(b));
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pair));
   rest = pack_half2(a - h.x, b - h.y);
 }
 
 // 16 dims d .. d + 15 (d a multiple of 16, below 64) and their partners 64
-// above, rotated: lo cos - hi sin, hi cos + lo sin; as fp16 pairs, and what those
-// round off.
-__device__ __forceinline__ void rotate16(const __half* row, uint32_t d, const DecodeParams& p,
-                                         uint32_t r, uint32_t* lo_out, uint32_t* hi_out,
-                                         uint32_t* lo_rest, uint32_t* hi_rest) {
+// above, rotated: lo cos - hi sin, hi cos + lo sin; as fp16 pairs.  SPLIT: and what
+// those round off; returns the 32 values' sum.
+template <bool SPLIT>
+__device__ __forceinline__ float rotate16(const __half* row, uint32_t d, const DecodeParams& p,
+                                          uint32_t r, uint32_t* lo_out, uint32_t* hi_out,
+                                          uint32_t* lo_rest, uint32_t* hi_rest) {
+  float sum = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; e += 4) {
     const uint2 lw = __ldg(reinterpret_cast<const uint2*>(row + d + e));
@@ -122,13 +128,22 @@ __device__ __forceinline__ void rotate16(const __half* row, uint32_t d, const De
       return __fadd_rn(__fmul_rn(x, c), __fmul_rn(y, s));
     };
     const int w = e / 2;
-    split2(turn(l0.x, cl.x, -h0.x, sl.x), turn(l0.y, cl.y, -h0.y, sl.y), lo_out[w], lo_rest[w]);
-    split2(turn(l1.x, cl.z, -h1.x, sl.z), turn(l1.y, cl.w, -h1.y, sl.w), lo_out[w + 1],
-           lo_rest[w + 1]);
-    split2(turn(h0.x, ch.x, l0.x, sh.x), turn(h0.y, ch.y, l0.y, sh.y), hi_out[w], hi_rest[w]);
-    split2(turn(h1.x, ch.z, l1.x, sh.z), turn(h1.y, ch.w, l1.y, sh.w), hi_out[w + 1],
-           hi_rest[w + 1]);
+    auto put = [&](float a, float b, uint32_t* out, uint32_t* rest) {
+      if (SPLIT) {
+        split2(a, b, *out, *rest);
+        sum += a + b;
+      } else {
+        *out = pack_half2(a, b);
+      }
+    };
+    put(turn(l0.x, cl.x, -h0.x, sl.x), turn(l0.y, cl.y, -h0.y, sl.y), lo_out + w, lo_rest + w);
+    put(turn(l1.x, cl.z, -h1.x, sl.z), turn(l1.y, cl.w, -h1.y, sl.w), lo_out + w + 1,
+        lo_rest + w + 1);
+    put(turn(h0.x, ch.x, l0.x, sh.x), turn(h0.y, ch.y, l0.y, sh.y), hi_out + w, hi_rest + w);
+    put(turn(h1.x, ch.z, l1.x, sh.z), turn(h1.y, ch.w, l1.y, sh.w), hi_out + w + 1,
+        hi_rest + w + 1);
   }
+  return sum;
 }
 
 // The low / high two code bytes of a word as an fp16 pair (exact).
@@ -155,6 +170,17 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1152.f));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Key codes: int8 ones with 1152 added, which costs no instruction to leave in and is taken
+// off the score as 1152 times the sum of q.  (Not so for values, whose sum over the rows cancels.)
+constexpr float KEY_BIAS = 1152.f;
+template <int CODE>
+__device__ __forceinline__ uint32_t key_lo(uint32_t w) {
+  return CODE == PVLC_KV8_E4M3 ? codes_lo<CODE>(w) : __byte_perm(w, 0x64646464u, 0x4140);
+}
+template <int CODE>
+__device__ __forceinline__ uint32_t key_hi(uint32_t w) {
+  return CODE == PVLC_KV8_E4M3 ? codes_hi<CODE>(w) : __byte_perm(w, 0x64646464u, 0x4342);
+}
 // A loaded word of codes as codes_lo / codes_hi take it.
 template <int CODE>
 __device__ __forceinline__ uint32_t biased(uint32_t w) {
@@ -173,8 +199,8 @@ struct Acc {
 // Scores of 32 keys (fragment row g of half tile mt is key 16 mt + pi(g), g + 8
 // eight above) into weights, with the running maximum; `live` keys count.
 template <int NT>
-__device__ __forceinline__ void weigh(float (&s)[2][NT][4], Acc<NT>& a, float kk, float lsv,
-                                      float rsv, int key0, int live, uint32_t (&w)[2][NT][2]) {
+__device__ __forceinline__ void weigh(float (&s)[2][NT][4], Acc<NT>& a, float kk,
+                                      const float (&off)[NT][2], float rsv, int key0, int live, uint32_t (&w)[2][NT][2]) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float t0 = -CUDART_INF_F, t1 = -CUDART_INF_F;
@@ -184,8 +210,8 @@ __device__ __forceinline__ void weigh(float (&s)[2][NT][4], Acc<NT>& a, float kk
       for (int r = 0; r < 2; ++r) {
         float* x = s[mt][nt] + 2 * r;
         const bool on = key0 + 16 * mt + 8 * r < live;
-        x[0] = on ? x[0] * kk + lsv : -CUDART_INF_F;
-        x[1] = on ? x[1] * kk + lsv : -CUDART_INF_F;
+        x[0] = on ? x[0] * kk + off[nt][0] : -CUDART_INF_F;
+        x[1] = on ? x[1] * kk + off[nt][1] : -CUDART_INF_F;
         t0 = fmaxf(t0, x[0]);
         t1 = fmaxf(t1, x[1]);
       }
@@ -231,7 +257,7 @@ __device__ __forceinline__ uint4 rest_words(const uint8_t* rest, int nt, int i) 
 template <int CODE, int NT>
 __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv, float qk,
                                           const uint32_t (&qf)[NT][16], const uint8_t* rest,
-                                          Acc<NT>& a, int g, int t) {
+                                          const float* bias, Acc<NT>& a, int g, int t) {
   const int pi = (g >> 1) | ((g & 1) << 2);
   float s[2][NT][4], low[2][NT][4];
 #pragma unroll
@@ -262,8 +288,8 @@ __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv,
         for (int mt = 0; mt < 2; ++mt) {
           const int i = 2 * f + e;
           const uint32_t ya = biased<CODE>(wa[mt][i]), yb = biased<CODE>(wb[mt][i]);
-          const uint32_t a0 = codes_lo<CODE>(ya), a1 = codes_lo<CODE>(yb);
-          const uint32_t a2 = codes_hi<CODE>(ya), a3 = codes_hi<CODE>(yb);
+          const uint32_t a0 = key_lo<CODE>(ya), a1 = key_lo<CODE>(yb);
+          const uint32_t a2 = key_hi<CODE>(ya), a3 = key_hi<CODE>(yb);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_16816(s[mt][nt], a0, a1, a2, a3, qf[nt][8 * j + 2 * i], qf[nt][8 * j + 2 * i + 1]);
@@ -279,7 +305,15 @@ __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv,
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[mt][nt][e] += low[mt][nt][e];
   uint32_t w[2][NT][2];
-  weigh<NT>(s, a, sk * qk, __log2f(sv), __frcp_rn(sv), 0, 64, w);
+  // t = s kk + log2(scale_V), less the keys' bias
+  const float kk = sk * qk, lsv = __log2f(sv);
+  float off[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      off[nt][c] = CODE == PVLC_KV8_E4M3 ? lsv : lsv - bias[nt * 8 + 2 * t + c] * kk;
+  weigh<NT>(s, a, kk, off, __frcp_rn(sv), 0, 64, w);
   // value rows t, t + 4, t + 8, t + 12 of a half tile: keys pi(2 t), pi(2 t + 1), ..
   const uint8_t* v = st + 4096;
 #pragma unroll
@@ -343,7 +377,8 @@ __device__ __forceinline__ void tail_tile(const uint8_t* kt, const uint8_t* vt, 
       }
   }
   uint32_t w[2][NT][2];
-  weigh<NT>(s, a, qk, 0.f, 1.f, pi, last + 1, w);
+  const float off[NT][2] = {};
+  weigh<NT>(s, a, qk, off, 1.f, pi, last + 1, w);
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -528,9 +563,9 @@ struct Units {
 };
 
 // A unit's rotated q as the consumers' fragments [NT][4][32 lanes] x 16 bytes, what it rounds
-// off in the same form, then its new key and value rows.
+// off in the same form, then its new key and value rows and each head's key bias (16 floats).
 template <int NT>
-constexpr uint32_t seq_slot() { return 2 * NT * 2048 + 512; }
+constexpr uint32_t seq_slot() { return 2 * NT * 2048 + 512 + 64; }
 
 template <int NT>
 constexpr uint32_t fixed_smem() {
@@ -739,13 +774,17 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       for (int nt = 0; nt < NT; ++nt) {
         uint32_t w[16], rest[16];
         const uint32_t head = nt * 8 + (lane >> 2);
+        float sum = 0.f;
         if (head < G) {
-          rotate16(p.q + (size_t)it.b * p.q_stride + ((size_t)it.h * G + head) * HD,
-                   16 * (lane & 3), p, it.sq.rope, w, w + 8, rest, rest + 8);
+          sum = rotate16<true>(p.q + (size_t)it.b * p.q_stride + ((size_t)it.h * G + head) * HD,
+                               16 * (lane & 3), p, it.sq.rope, w, w + 8, rest, rest + 8);
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) w[e] = rest[e] = 0;
         }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if ((lane & 3) == 0) reinterpret_cast<float*>(slot + 2 * NT * 2048 + 512)[head] = KEY_BIAS * sum;
         uint4* to = reinterpret_cast<uint4*>(slot) + nt * 128 + lane;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -759,9 +798,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         uint4* kn = reinterpret_cast<uint4*>(slot + 2 * NT * 2048);
         uint4* vn = kn + 16;
         if (lane < 4) {
-          uint32_t w[16], rest[16];
-          rotate16(p.k_new + (size_t)it.b * p.kv_stride + it.h * HD, 16 * lane, p, it.sq.rope, w,
-                   w + 8, rest, rest + 8);
+          uint32_t w[16];
+          rotate16<false>(p.k_new + (size_t)it.b * p.kv_stride + it.h * HD, 16 * lane, p,
+                          it.sq.rope, w, w + 8, nullptr, nullptr);
           uint4* row = reinterpret_cast<uint4*>(tail_rows(p.c, it.sq.slot, 0, it.h) + last * HD);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -904,7 +943,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           seek(at + i - i0 + skew);
           if (landed()) {
             const float2 sc = scale[stage];
-            page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, slot + NT * 2048, a, g, t);
+            page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, slot + NT * 2048,
+                                reinterpret_cast<const float*>(slot + 2 * NT * 2048 + 512), a, g, t);
           }
           release(stage);
         }

@@ -372,6 +372,11 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_compact_plan_kernel(const
     const int32_t n = c.a.tokens[s];
     if (n < 0 || !rows_fit((uint32_t)n, c.to_max_pages)) wide = 1;
   }
+  if (c.a.max_pages > c.to_max_pages) {  // nor may a page for later rows be left behind
+    const uint64_t more = c.a.max_pages - c.to_max_pages;
+    for (uint64_t i = threadIdx.x; i < c.a.slots * more; i += PLAN_THREADS)
+      if (c.a.table[i / more * c.a.max_pages + c.to_max_pages + i % more] >= 0) wide = 1;
+  }
   wide = __syncthreads_or(wide);
   if (threadIdx.x == 0) {
     const bool fits = count <= c.to_pages && !wide;

@@ -239,6 +239,28 @@ def test_decode_many_ragged(kv8, code):
 def test_decode_flat_and_peaked_scores(kv8, scale_q):
     """All scores equal, and scores so far apart that one row takes all the weight."""
     decode_case(kv8, "e4m3", [100, 1000, 31], 2, 8, seed=10, scale_q=scale_q)
+    decode_case(kv8, "int8", [100, 1000, 31], 2, 8, seed=10, scale_q=scale_q)
+
+
+def test_decode_query_beyond_half_precision(kv8):
+    """A rotated q beyond fp16's range (60000 sqrt(2)): the cached keys are scaled down so that
+    the scores stay ordinary."""
+    lengths = [70, 33]
+    c = R.filled_cache(kv8, "e4m3", lengths, 2, seed=18, spare=4)
+    c.scales[..., 0] *= 2.0 ** -15
+    q = torch.full((2, 16, 128), 60000.0, device="cuda").half()
+    kv = torch.zeros((2, 2, 128), device="cuda").half()
+    c.tails.zero_()
+    cos, sin = R.rope_tables(100)
+    ref = R.Ref(c, "e4m3")
+    ws = kv8.Workspace(c, 2, 16)
+    out = kv8.decode(c, 0, q, kv, kv, torch.from_numpy(cos).cuda(), torch.from_numpy(sin).cuda(),
+                     None, ws).cpu().numpy()
+    hq, hkv = q.cpu().numpy(), kv.cpu().numpy()
+    for b in range(2):
+        want, tol = ref.decode(0, b, hq[b], hkv[b], hkv[b], cos, sin, lengths[b])
+        assert np.isfinite(out[b]).all() and (np.abs(out[b] - want) <= tol).all()
+    assert ws.errors() == 0
 
 
 @pytest.mark.parametrize("code", CODES)
@@ -528,7 +550,7 @@ def test_compact(kv8, code, layers, pages):
 
 
 def test_compact_that_does_not_fit(kv8):
-    c = R.filled_cache(kv8, "e4m3", [40, 200], 2, seed=27)
+    c = R.filled_cache(kv8, "e4m3", [40, 200], 2, seed=27, spare=4)   # 2 + 2 pages for 60 rows
     ws = kv8.Workspace(c, 2)
     n = torch.zeros(1, dtype=torch.int32, device="cuda")
     for spare, room, flag in ((6, 9, kv8.FLAG_EXHAUSTED), (9, 5, kv8.FLAG_ROWS_HELD)):
@@ -538,6 +560,13 @@ def test_compact_that_does_not_fit(kv8):
         kv8.compact(c, into, ws, live=n)
         assert int(n) == -1 and ws.errors() == flag
         ref.same(into)
+    # a page given for later rows that the narrower table has no room for
+    into = R.filled_cache(kv8, "e4m3", [3] * 2, 2, seed=28, spare=20, room=7, poison=False)
+    ref = R.Ref(into, "e4m3")
+    kv8.grow(c, ints([0, 1]), ws, ahead=60)
+    kv8.compact(c, into, ws, live=n)
+    assert int(n) == -1 and ws.errors() == kv8.FLAG_ROWS_HELD
+    ref.same(into)
 
 
 # --------------------------------------------------------------- wrappers
