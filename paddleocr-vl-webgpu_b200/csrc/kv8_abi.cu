@@ -38,6 +38,20 @@ int check_cache(const pvlc_kv8_cache* c) {
   return PVLC_OK;
 }
 
+// The byte ranges of a cache's arrays.
+struct Ranges {
+  uintptr_t at[6];
+  uint64_t bytes[6];
+};
+Ranges ranges(const pvlc_kv8_cache& c) {
+  const uint64_t heads = (uint64_t)c.layers * c.kv_heads, block = PVLC_KV8_PAGE * 128;
+  return {{reinterpret_cast<uintptr_t>(c.codes), reinterpret_cast<uintptr_t>(c.scales),
+           reinterpret_cast<uintptr_t>(c.tails), reinterpret_cast<uintptr_t>(c.table),
+           reinterpret_cast<uintptr_t>(c.tokens), reinterpret_cast<uintptr_t>(c.refs)},
+          {heads * c.pages * 2 * block, heads * c.pages * 8, heads * c.slots * 4 * block,
+           (uint64_t)c.slots * c.max_pages * 4, (uint64_t)c.slots * 4, (uint64_t)c.pages * 4}};
+}
+
 size_t page_scratch(uint32_t batch, uint32_t slots, uint32_t pages) {
   const size_t fork = 4 + 6 * (size_t)batch + slots, compact = 4 + 2 * (size_t)pages;
   return 4 * (fork > compact ? fork : compact);
@@ -200,6 +214,11 @@ int pvlc_attn_kv8_compact(const pvlc_kv8_cache* from, const pvlc_kv8_cache* into
   if (!aligned(live_out, 4)) return PVLC_MISALIGNED_POINTER;
   if ((st = check_workspace(workspace, workspace_bytes, page_scratch(1, from->slots, from->pages))))
     return st;
+  const Ranges a = ranges(*from), b = ranges(*into);
+  for (int i = 0; i < 6; ++i)
+    for (int j = 0; j < 6; ++j)
+      if (a.at[i] < b.at[j] + b.bytes[j] && b.at[j] < a.at[i] + a.bytes[i])
+        return PVLC_LENGTH_MISMATCH;       // nor parts of them
   return kv8_compact_launch(*from, *into, live_out, workspace, static_cast<cudaStream_t>(stream));
 }
 

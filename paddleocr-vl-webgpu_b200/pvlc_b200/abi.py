@@ -132,11 +132,26 @@ _SIGNATURES = {
 EXPORTED = tuple(_SIGNATURES)
 
 _lib = None
+# The compiled argument checks of the 8-bit cache's calls (csrc/py_calls.cpp), once the library
+# is loaded; None where they were not built for this Python and torch: the checks in Python
+# then make the same calls, each about 10 us later.
+calls = None
+
+
+def _bind_calls(handle):
+    try:
+        from . import _calls
+    except ImportError:
+        return None
+    _calls.bind(*[ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in
+                  ("pvlc_attn_kv8_store", "pvlc_attn_kv8_decode", "pvlc_attn_kv8_grow",
+                   "pvlc_attn_kv8_fork", "pvlc_attn_kv8_compact", "pvlc_lm_head_beam_topk")])
+    return _calls
 
 
 def lib() -> ctypes.CDLL:
     """Load the in-tree CUDA library (raises if it has not been built)."""
-    global _lib
+    global _lib, calls
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"{LIB_PATH} is missing: build it with __graft_entry__.build() "
@@ -147,6 +162,7 @@ def lib() -> ctypes.CDLL:
             fn.restype = res
             fn.argtypes = args
         _lib = handle
+        calls = _bind_calls(handle)
     return _lib
 
 

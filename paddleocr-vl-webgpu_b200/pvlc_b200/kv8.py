@@ -176,6 +176,15 @@ def _call(cache, workspace):
     return index
 
 
+# Each function below first hands its arguments to the compiled checks (csrc/py_calls.cpp),
+# which make the call when all is well and return None otherwise; then the checks here run
+# and name what is wrong (or make the call, for what those do not know, a tensor subclass).
+
+
+def _plain(cache, workspace):
+    return abi.calls is not None and type(cache) is Cache and type(workspace) is Workspace
+
+
 def store(cache: Cache, layer: int, k, v, begin, count, slot, max_count: int,
           workspace: Workspace):
     """Append rows to sequences in one layer (pvlc_attn_kv8_store).
@@ -183,6 +192,11 @@ def store(cache: Cache, layer: int, k, v, begin, count, slot, max_count: int,
     k, v: [rows, kv_heads, 128] fp16, keys rotated, rows the same distance apart in both;
     sequence b takes rows begin[b] : begin[b] + count[b] (int32 device tensors, count <=
     max_count) behind the rows its slot holds."""
+    if _plain(cache, workspace):
+        st = abi.calls.store(cache._p, cache.index, workspace._p, workspace.nbytes,
+                             workspace.index, layer, slot, k, v, begin, count, max_count)
+        if st is not None:
+            return abi.check(st, "pvlc_attn_kv8_store")
     index = _call(cache, workspace)
     n, stride = _rows(k, cache.kv_heads, index, "k")
     if _rows(v, cache.kv_heads, index, "v") != (n, stride):
@@ -191,7 +205,7 @@ def store(cache: Cache, layer: int, k, v, begin, count, slot, max_count: int,
     _need(slot, torch.int32, (B,), index, "slot")
     _need(begin, torch.int32, (B,), index, "begin")
     _need(count, torch.int32, (B,), index, "count")
-    if not 0 <= layer < cache.layers or max_count < 0:
+    if not 0 <= layer < cache.layers or not 0 <= max_count < 1 << 32:
         raise ValueError("layer or max_count out of range")
     st = abi.lib().pvlc_attn_kv8_store(
         cache._p, layer, k.data_ptr(), v.data_ptr(), n, stride, begin.data_ptr(),
@@ -210,6 +224,14 @@ def decode(cache: Cache, layer: int, q, k_new, v_new, rope_cos, rope_sin, slot,
     row-strided view (column blocks of one projection; k_new and v_new alike); rope tables
     [3, R, 128] f32; rope_row int32 [B] (None: the rows the slot holds); slot int32 [B] (None:
     sequence b is slot b).  Returns [B, query_heads, 128] fp16."""
+    if _plain(cache, workspace):
+        r = abi.calls.decode(cache._p, cache.index, workspace._p, workspace.nbytes,
+                             workspace.index, layer, q, k_new, v_new, rope_cos, rope_sin, slot,
+                             rope_row, out)
+        if type(r) is int:
+            abi.check(r, "pvlc_attn_kv8_decode")
+        if r is not None:
+            return r
     index, H = _call(cache, workspace), cache.kv_heads
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise TypeError("q must be a [B, query_heads, 128] CUDA tensor")
@@ -257,6 +279,11 @@ def _amount(x, B, index, name):
 def grow(cache: Cache, slot, workspace: Workspace, advance=0, ahead=0):
     """Advance sequences by `advance` rows and give them the pages of their next `ahead` rows
     (each a number, or an int32 tensor per sequence; pvlc_attn_kv8_grow)."""
+    if _plain(cache, workspace):
+        st = abi.calls.grow(cache._p, cache.index, workspace._p, workspace.nbytes,
+                            workspace.index, slot, advance, ahead)
+        if st is not None:
+            return abi.check(st, "pvlc_attn_kv8_grow")
     index, B = _call(cache, workspace), _batch(slot)
     _need(slot, torch.int32, (B,), index, "slot")
     ap, an = _amount(advance, B, index, "advance")
@@ -270,6 +297,13 @@ def grow(cache: Cache, slot, workspace: Workspace, advance=0, ahead=0):
 def fork(cache: Cache, slot, parent, workspace: Workspace, advance: int = 0, out=None):
     """Sequence b becomes a copy of sequence parent[b] (int32 [B], -1: none), after every
     sequence has grown by `advance` rows; returns the new slots (pvlc_attn_kv8_fork)."""
+    if _plain(cache, workspace):
+        r = abi.calls.fork(cache._p, cache.index, workspace._p, workspace.nbytes,
+                           workspace.index, slot, parent, advance, out)
+        if type(r) is int:
+            abi.check(r, "pvlc_attn_kv8_fork")
+        if r is not None:
+            return r
     index, B = _call(cache, workspace), _batch(slot)
     _need(slot, torch.int32, (B,), index, "slot")
     _need(parent, torch.int32, (B,), index, "parent")
@@ -291,6 +325,11 @@ def compact(cache: Cache, into: Cache, workspace: Workspace, live=None):
     """Copy the live pages, in order, to the front of another cache with the same layers,
     heads and type, and make its tables match (pvlc_attn_kv8_compact).  live: optional int32
     [1] tensor that receives the number of live pages (-1: they do not fit)."""
+    if _plain(cache, workspace) and type(into) is Cache:
+        st = abi.calls.compact(cache._p, cache.index, workspace._p, workspace.nbytes,
+                               workspace.index, into._p, into.index, live)
+        if st is not None:
+            return abi.check(st, "pvlc_attn_kv8_compact")
     index = _call(cache, workspace)
     if not isinstance(into, Cache):
         raise TypeError("into must be a kv8.Cache")

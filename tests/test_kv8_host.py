@@ -195,6 +195,38 @@ def test_beam_refusals(change, code):
         assert abi.lib().pvlc_lm_head_beam_topk_workspace_bytes(a["B"], a["W"], a["V"], a["K"]) == 0
 
 
+def test_compact_refuses_overlapping_caches():
+    """No array of one cache may share bytes with any of the other."""
+    f = abi.lib().pvlc_attn_kv8_compact
+    names = ("codes", "scales", "tails", "table", "tokens", "refs")
+    step = 1 << 30                         # more than any array of the two holds
+    a = cache(**{n: step * (i + 1) for i, n in enumerate(names)})
+    b = {n: step * (i + 7) for i, n in enumerate(names)}
+    for i, n in enumerate(names):
+        for m in names:
+            # 16 bytes into one of a's arrays (each is longer than that)
+            at = step * (i + 1) + 16
+            assert f(ctypes.byref(a), ctypes.byref(cache(**{**b, m: at})), None, P16, BIG,
+                     None) == abi.LENGTH_MISMATCH, (n, m)
+
+
+def test_compiled_checks_pass_nothing_by_on_the_host():
+    """The compiled argument checks were built, and hand anything that is not a CUDA call back
+    to the Python ones (None)."""
+    abi.lib()
+    c = abi.calls
+    assert c is not None, "make -C paddleocr-vl-webgpu_b200 builds pvlc_b200/_calls.so"
+    t, i = torch.zeros((2, 2, 128), dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
+    head = (0, 0, 0, 0, 0)
+    for args in ((), (None,), head, (*head, 0, i, t, t, i, i, 4), (*head, -1, i, t, t, i, i, 4),
+                 (*head, 0, t, t, t, t, t, i, None, None), (*head, i, i, i, None),
+                 (*head, i, 1, 1), (1 << 70, *head[1:], i, 1, 1), (*head, 0, 0, None), ("x",) * 14,
+                 (torch.zeros((2, 9)), torch.zeros((1, 2)), 2, torch.zeros(64, dtype=torch.uint8)),
+                 (i, i, 2, i), (None, None, None, None)):
+        for fn in (c.store, c.decode, c.grow, c.fork, c.compact, c.beam_topk):
+            assert fn(*args) is None, (fn, args)
+
+
 def test_wrappers_refuse_host_tensors():
     t = torch.zeros((1, 4, 2, 2, 32, 128), dtype=torch.int8)
     with pytest.raises(TypeError):
