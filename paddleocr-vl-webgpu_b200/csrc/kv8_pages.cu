@@ -10,7 +10,12 @@
 // sums, and the reference counts are integer sums.
 //
 // Deciding is one block's work (a few thousand integers); the copies that
-// follow are spread over the GPU.
+// follow are spread over the GPU.  Measured, 18 layers of 2 heads, calls back to back:
+//   fork and grow of 2 x 4 beams 9 us, of 64 x 4 beams 19 us (44 MB of open rows, 6.7 us of
+//     a copy's rate; the rest is three launches, each a chain of dependent loads and scans,
+//     that wait for one another)
+//   compact of 32 sequences, 951 MB read and written, 166 us (5.7 TB/s, 87 % of a copy); of
+//     65 pages 8.7 us, two launches
 #include <cuda_runtime.h>
 
 #include "kv8.cuh"
@@ -282,7 +287,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const Fo
   }
 }
 
-// A warp copies the open rows of one (copy, layer, K or V, head); a block does the
+// A warp copies the open rows of one (copy, layer, K or V, head), up to 8 KB, four loads a lane
+// at a time: 9 us of the 19 above, a copy's rate while it runs and latency around it.  A block does the
 // table row, count and page references of one touched slot.  A source slot is a
 // kept one and a destination is not, so nothing is read that another one writes.
 __global__ void __launch_bounds__(COPY_THREADS) kv8_fork_copy_kernel(const ForkParams f) {
@@ -390,6 +396,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_compact_plan_kernel(const
 // bulk copy in and one out, so that no registers or load slots bound the bytes in
 // flight: two warps of 12 lanes, a stage each, 192 KB an SM.  The two warps' reads
 // and writes alternate against each other.  The other warps do the small things.
+// 32 sequences: 166 us, with loads and stores through registers 174.
 constexpr uint32_t PIECE = 2 * BLOCK_CODES;
 constexpr uint32_t LANES = 12, ENGINES = 2;
 constexpr uint32_t COMPACT_SMEM = LANES * ENGINES * (PIECE + 8);
