@@ -407,7 +407,16 @@ int pvlc_linear(const pvlc_half* x, uint32_t rows, uint32_t ldx, const pvlc_half
  * those a page that the next blocks will fill, or -1.  refs[p] counts the
  * slots that name page p; 0 is a free page.  A cache starts with table -1,
  * tokens and refs 0.  A slot with 0 tokens that no call names is free.
- * head_dim is 128.  Every call takes sequences as `slot[batch]`: distinct slots,
+ * head_dim is 128.
+ *
+ * Ordering: each of these calls waits for the kernels ahead of it on `stream`
+ * before it reads or writes anything, and lets the kernel behind it start
+ * early, as all of them allow.  So what they write (tokens, slots, tokens of a
+ * selection) may be read by any call behind them but, directly behind, by one that
+ * reads before it waits: pvlc_attn_decode's cache_tokens and rope_row, pvlc_linear's
+ * weights.
+ *
+ * Every call takes sequences as `slot[batch]`: distinct slots,
  * or -1 for an idle sequence, which is passed over (its outputs are left as
  * they were).  All arrays are device memory; the struct itself is read during
  * the call only.
@@ -434,7 +443,8 @@ typedef struct pvlc_kv8_cache {
 /* Scratch of the kv8 calls on caches of up to `pages` pages and `slots` slots,
  * for batches of up to `batch` sequences and `query_heads` heads (0 when they
  * are out of range).  Zeroed once with pvlc_attn_kv8_workspace_init; reusable
- * on one stream, not by calls that may overlap.  pvlc_attn_kv8_errors waits
+ * on one stream, not by calls that may overlap.  After bit 3 it has to be
+ * initialised again.  pvlc_attn_kv8_errors waits
  * for the stream, reads and clears the fault word: bit 0 a slot's row count or
  * capacity, bit 1 a rope row, bit 3 a pipeline wait that timed out, bit 4 a
  * page id, bit 5 a slot or parent, bit 6 no free page or slot, bit 7 the

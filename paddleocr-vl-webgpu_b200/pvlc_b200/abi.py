@@ -140,6 +140,8 @@ calls = None
 
 def _bind_calls(handle):
     try:
+        import torch  # noqa: F401  (its libraries are what the module links against)
+
         from . import _calls
     except ImportError:
         return None

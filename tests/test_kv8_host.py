@@ -227,6 +227,17 @@ def test_compiled_checks_pass_nothing_by_on_the_host():
             assert fn(*args) is None, (fn, args)
 
 
+def test_compiled_checks_load_in_a_fresh_process():
+    """Also where the library is loaded before anything has imported torch."""
+    import os
+    import subprocess
+    import sys
+    package = os.path.dirname(os.path.dirname(abi.__file__))
+    code = f"import sys; sys.path.insert(0, {package!r}); from pvlc_b200 import abi; abi.lib(); " \
+           "sys.exit(abi.calls is None)"
+    assert subprocess.run([sys.executable, "-c", code]).returncode == 0
+
+
 def test_wrappers_refuse_host_tensors():
     t = torch.zeros((1, 4, 2, 2, 32, 128), dtype=torch.int8)
     with pytest.raises(TypeError):
