@@ -18,13 +18,19 @@
 // group of 8.  That is 1 % of the tensor cores' rate, so mma.sync on registers,
 // which needs no second copy of the codes, is enough (their pipe is active 15 % of
 // the time).  Measured, a layer of 16 query and 2 KV heads, calls back to back:
-//   64 sequences of 606 .. 8,011 rows   34.7 us   4.2 TB/s, 64 % of a copy
+//   64 sequences of 606 .. 8,011 rows   34.5 us   4.2 TB/s, 65 % of a copy
 //   16 sequences, 8 KV heads, 4 k .. 8 k rows   38.3 us   4.7 TB/s, 72 %
-//   64 x 4 beams of 1,238 .. 1,499 rows   45.1 us   190 MB through L2, 55 MB of them distinct
-//   1 sequence of 1,023 rows   10.3 us   bound by its chain of dependent loads
-// Of the 34.7 us about 21 are the stream at a copy's rate; 4.3 pass before the
-// first page lands (launch, the sequences' slots, lengths and page ids, each read
-// after the other), the rest is the uneven end and the join of the split units.
+//   64 x 4 beams of 1,248 .. 1,499 rows   44.9 us   190 MB through L2, 55 MB of them distinct
+//   1 sequence of 1,023 rows   10.0 us   bound by its chain of dependent loads
+// Of the 34.5 us 22.3 are the stream at a copy's rate.  4 pass before the first
+// page lands (launch, the sequences' slots, lengths and page ids, each read after
+// the other), 3 in joining the split units, the rest in the uneven end: without
+// its arithmetic the kernel takes 32.3, without its pages 29.4.  The beams are
+// bound by the warps' arithmetic, a page's 48 matrix and some 350 other
+// instructions: 32.9 and 42.1 (int8, whose conversions are byte permutations).
+// More warps an SM do not help (5, 6 and 8 a block: 49, 48 and 56), nor does
+// loading a page that four beams share once, a warp a beam (65: the same work in
+// more code).
 // What the design does about it:
 //   * The (sequence, KV head) units, each its pages and a tail, are laid end to
 //     end with an allowance for a unit's end, and cut into equal ranges, one per
@@ -63,8 +69,8 @@
 namespace pvlc {
 namespace kv8 {
 
-// Consumer warps: two blocks of 4 an SM fill its registers.  64 ragged sequences took 41.8 us
-// with 4 and 42.5 with 6, when both were tried.
+// Consumer warps: two blocks of 4 an SM fill its registers.  64 ragged sequences take
+// 34.8 us with 4, 37.5 with 5, 36.8 with 6, 46.2 with 8.
 constexpr int WARPS = 4;
 constexpr int THREADS = (WARPS + 2) * 32;         // + the producer and the sequence warp
 constexpr int CTHREADS = WARPS * 32;
@@ -493,8 +499,15 @@ __device__ __forceinline__ void join_head(const float* records, const Split& u, 
       }
   };
   load(0);
-  float m = -CUDART_INF_F;
-  for (uint32_t c = sub; c < n; c += 8) m = fmaxf(m, __ldcg(record(c) + 8 * NT * HD + i));
+  // lane `sub` keeps the maximum and the sum of record `sub`; a unit of more than 8 asks again
+  float m_own = -CUDART_INF_F, l_own = 0.f;
+  if (sub < n) {
+    const float* r = record(sub) + 8 * NT * HD + i;
+    m_own = __ldcg(r);
+    l_own = __ldcg(r + 8 * NT);
+  }
+  float m = m_own;
+  for (uint32_t c = sub + 8; c < n; c += 8) m = fmaxf(m, __ldcg(record(c) + 8 * NT * HD + i));
 #pragma unroll
   for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float l = 0.f;
@@ -504,17 +517,18 @@ __device__ __forceinline__ void join_head(const float* records, const Split& u, 
   // the lanes of a warp may have units of different spans: they stay together
   const uint32_t most = __reduce_max_sync(0xffffffffu, n);
   for (uint32_t base = 0; base < most; base += R) {
-    float f = 0.f, fl = 0.f;
-    if (sub < R && base + sub < n) {
+    if (base && base % 8 == 0 && base + sub < n) {
       const float* r = record(base + sub) + 8 * NT * HD + i;
-      f = fast_exp2(__ldcg(r) - m);
-      fl = __ldcg(r + 8 * NT) * f;
+      m_own = __ldcg(r);
+      l_own = __ldcg(r + 8 * NT);
     }
+    const float f = base / 8 * 8 + sub < n ? fast_exp2(m_own - m) : 0.f, fl = f * l_own;
 #pragma unroll
     for (int e = 0; e < R; ++e) {
-      const float fe = __shfl_sync(0xffffffffu, f, e, 8);
-      l += __shfl_sync(0xffffffffu, fl, e, 8);
+      const float fe = __shfl_sync(0xffffffffu, f, base % 8 + e, 8);
+      const float le = __shfl_sync(0xffffffffu, fl, base % 8 + e, 8);
       if (base + e < n) {
+        l += le;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           o[d].x += x[e][d].x * fe;
