@@ -310,6 +310,8 @@ def generate(eng, images_patches, grids, max_new_tokens, beams, length_penalty, 
     es, en, eb, done, live = (h.numpy() for h, _ in ends)
     found = [hypotheses(tok[:, r], beam[:, r], es[r], en[r], eb[r], bool(done[r]), live[r],
                         length_penalty) for r in range(B)]
+    if not all(found):                      # every logit of some request NaN or -infinity
+        raise greedy.GreedyError(greedy.NON_FINITE_INPUT, "no hypothesis has a finite score")
     found = [[(s, p + [c.eos_token_id] if why == greedy.EOS_TOKEN else p, why)
               for s, p, why in f] for f in found]
     if ev:

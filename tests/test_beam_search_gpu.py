@@ -251,3 +251,16 @@ def test_refusals(setup):
         eng.generate_beam(patches, GRIDS, 0)
     with pytest.raises(TypeError):
         eng.generate_beam(patches, GRIDS, 4, cache_dtype=torch.float16)
+
+
+def test_non_finite_logits_are_an_error(setup):
+    """As in the greedy search; the engine is of use again afterwards."""
+    w, patches = setup
+    eng = M.OcrEngine(CFG, w)
+    good = eng.generate_beam(patches, GRIDS, 4, beams=2)
+    head, eng.lm_head = eng.lm_head, torch.full_like(eng.lm_head, math.nan)
+    eng._beam = None                     # the captured step reads the head that it was captured with
+    with pytest.raises(greedy.GreedyError):
+        eng.generate_beam(patches, GRIDS, 4, beams=2)
+    eng.lm_head, eng._beam = head, None
+    assert eng.generate_beam(patches, GRIDS, 4, beams=2) == good
