@@ -431,16 +431,20 @@ __device__ __forceinline__ void tail_tile(const uint8_t* kt, const uint8_t* vt, 
   }
 }
 
-// The block whose cost range holds position y of a line of C cut into G.
-__device__ __forceinline__ uint32_t owner_of(uint64_t y, uint64_t G, uint64_t C) {
-  return static_cast<uint32_t>(((y + 1) * G + C - 1) / C - 1);
-}
-
-// floor(i C / N): where block i's range begins.
-__device__ __forceinline__ uint64_t cut_at(uint64_t i, uint64_t C, uint64_t N) {
-  const uint64_t x = i * C;
-  return x >> 32 ? x / N : (uint32_t)x / (uint32_t)N;
-}
+// A line of C cut into N ranges, the first `more` of them one longer than `each`.
+struct Cuts {
+  uint64_t each;
+  uint32_t more;
+  __device__ __forceinline__ Cuts(uint64_t C, uint32_t N) {
+    each = C >> 32 ? C / N : (uint32_t)C / N;
+    more = (uint32_t)(C - each * N);
+  }
+  __device__ __forceinline__ uint64_t begin(uint32_t i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ uint32_t owner(uint64_t y) const {      // the range that y is in
+    const uint64_t longer = more * (each + 1);
+    return (uint32_t)(y < longer ? y / (each + 1) : more + (y - longer) / each);
+  }
+};
 
 struct Seq {
   uint32_t cost;     // cost position of the sequence's first unit, per KV head
@@ -683,13 +687,18 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
   if (C == 0) return;
   const uint64_t N = C / MIN_COST >= gridDim.x ? gridDim.x : umax64(1, C / MIN_COST);
   if (blockIdx.x >= N) return;
-  const uint64_t y0 = cut_at(blockIdx.x, C, N), y1 = cut_at(blockIdx.x + 1, C, N);
-  // the last sequence whose line starts at or before y (idle ones have no length)
+  const Cuts cuts(C, (uint32_t)N);
+  const uint64_t y0 = cuts.begin(blockIdx.x), y1 = cuts.begin(blockIdx.x + 1);
+  // the last sequence whose line starts at or before y (idle ones have no length); a warp
+  // looks at 32 places at once
   auto seq_at = [&](uint64_t y) -> uint32_t {
-    uint32_t lo = 0, hi = B;
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if ((uint64_t)seq[mid].cost * H <= y) lo = mid; else hi = mid;
+    uint32_t lo = 0, n = B;              // it is one of [lo, lo + n)
+    while (n > 1) {
+      const uint32_t step = (n + 31) / 32, off = lane * step;
+      const bool before = off < n && (uint64_t)seq[lo + off].cost * H <= y;
+      const uint32_t skip = (__popc(__ballot_sync(0xffffffffu, before)) - 1) * step;
+      lo += skip;
+      n = min(step, n - skip);
     }
     return lo;
   };
@@ -849,11 +858,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       }
       if (lane == 0 && !it.whole()) {
         // the unit spans blocks c0 .. c1: it is the last one of c0, the first of the others
-        const uint32_t c0 = owner_of(it.u0, N, C), c1 = owner_of(it.u0 + it.np, N, C);
+        const uint32_t c0 = cuts.owner(it.u0), c1 = cuts.owner(it.u0 + it.np);
         Split& u = splits[it.u0 >= y0 ? 1 : 0];
         u.unit = it.b * H + it.h;
         u.blocks = c1 - c0 + 1;
-        u.record = c0 * 2 + (it.u0 >= cut_at(c0, C, N) ? 1 : 0);
+        u.record = c0 * 2 + (it.u0 >= cuts.begin(c0) ? 1 : 0);
       }
       mbar_arrive(row_full + s);
       if (it.has_tail() && it.sq.rows % PAGE == PAGE - 1) {
