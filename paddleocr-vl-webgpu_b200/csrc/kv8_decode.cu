@@ -18,11 +18,11 @@
 // group of 8.  That is 1 % of the tensor cores' rate, so mma.sync on registers,
 // which needs no second copy of the codes, is enough (their pipe is active 15 % of
 // the time).  Measured, a layer of 16 query and 2 KV heads, calls back to back:
-//   64 sequences of 606 .. 8,011 rows   34.5 us   4.2 TB/s, 65 % of a copy
-//   16 sequences, 8 KV heads, 4 k .. 8 k rows   38.3 us   4.7 TB/s, 72 %
+//   64 sequences of 606 .. 8,011 rows   34.3 us   4.3 TB/s, 65 % of a copy
+//   16 sequences, 8 KV heads, 4 k .. 8 k rows   37.9 us   4.8 TB/s, 72 %
 //   64 x 4 beams of 1,248 .. 1,499 rows   44.9 us   190 MB through L2, 55 MB of them distinct
-//   1 sequence of 1,023 rows   10.0 us   bound by its chain of dependent loads
-// Of the 34.5 us 22.3 are the stream at a copy's rate.  4 pass before the first
+//   1 sequence of 1,023 rows   9.9 us   bound by its chain of dependent loads
+// Of the 34.3 us 22.3 are the stream at a copy's rate.  4 pass before the first
 // page lands (launch, the sequences' slots, lengths and page ids, each read after
 // the other), 3 in joining the split units, the rest in the uneven end: without
 // its arithmetic the kernel takes 32.3, without its pages 29.4.  The beams are
