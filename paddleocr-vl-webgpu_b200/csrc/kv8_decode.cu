@@ -15,7 +15,7 @@
 // so the codes go to the tensor cores as the fp16 numbers they are.
 //
 // Bound by HBM: 2 x 128 bytes a row and KV head, 16 operations a byte at a
-// group of 8.  That is 1 % of the tensor cores' rate, so mma.sync on registers,
+// group of 8.  That is 6 % of the tensor cores' rate, so mma.sync on registers,
 // which needs no second copy of the codes, is enough (their pipe is active 15 % of
 // the time).  Measured, a layer of 16 query and 2 KV heads, calls back to back:
 //   64 sequences of 606 .. 8,011 rows   34.3 us   4.3 TB/s, 65 % of a copy
@@ -26,8 +26,9 @@
 // page lands (launch, the sequences' slots, lengths and page ids, each read after
 // the other), 3 in joining the split units, the rest in the uneven end: without
 // its arithmetic the kernel takes 32.3, without its pages 29.4.  The beams are
-// bound by the warps' arithmetic, a page's 48 matrix and some 350 other
-// instructions: 32.9 and 42.1 (int8, whose conversions are byte permutations).
+// bound by the warps' arithmetic, a page's 48 matrix and some 600 other
+// instructions, each waiting for the one ahead of it more than for a pipe: 32.9
+// and 42.1 (int8, whose conversions are byte permutations).
 // More warps an SM do not help (5, 6 and 8 a block: 49, 48 and 56), nor does
 // loading a page that four beams share once, a warp a beam (65: the same work in
 // more code).

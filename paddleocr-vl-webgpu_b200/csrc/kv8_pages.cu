@@ -11,8 +11,8 @@
 //
 // Deciding is one block's work (a few thousand integers); the copies that
 // follow are spread over the GPU.  Measured, 18 layers of 2 heads, calls back to back:
-//   fork and grow of 2 x 4 beams 9 us, of 64 x 4 beams 19 us (44 MB of open rows, 6.7 us of
-//     a copy's rate; the rest is three launches, each a chain of dependent loads and scans,
+//   fork and grow of 2 x 4 beams 8.9 us, of 64 x 4 beams 17.7 us (44 MB of open rows, 6.7 us
+//     of a copy's rate; the rest is three launches, each a chain of dependent loads and scans,
 //     that wait for one another)
 //   compact of 32 sequences, 951 MB read and written, 166 us (5.7 TB/s, 87 % of a copy); of
 //     65 pages 8.7 us, two launches
@@ -62,10 +62,12 @@ struct PageParams {
 };
 
 // Copies the slots to shared memory; whether each is idle (-1) or in range, and
-// none is named twice.  `seen` is a bitmap over the slots in shared memory.
-__device__ bool slots_valid(const PageParams& p, uint32_t* seen, int32_t* slot) {
+// none is named twice.  `seen` is a bitmap over the slots in shared memory, `first`
+// this thread's slot of the first PLAN_THREADS, which its caller has asked for early.
+__device__ bool slots_valid(const PageParams& p, uint32_t* seen, int32_t* slot, int32_t first) {
   for (uint32_t i = threadIdx.x; i < (p.slots + 31) / 32; i += PLAN_THREADS) seen[i] = 0;
-  for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) slot[b] = p.slot[b];
+  for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS)
+    slot[b] = b == threadIdx.x ? first : p.slot[b];
   __syncthreads();
   int bad = 0;
   for (uint32_t b = threadIdx.x; b < p.batch; b += PLAN_THREADS) {
@@ -96,7 +98,17 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
   int32_t* slot = reinterpret_cast<int32_t*>(sm);
   pdl_wait();
   pdl_launch_dependents();
-  int bad = slots_valid(p, sm + p.batch, slot) ? 0 : (int)kFlagSlot;
+  // the slots and the first pages' counts at once, although few calls need the latter
+  const int32_t first = threadIdx.x < p.batch ? p.slot[threadIdx.x] : -1;
+  auto free_pages = [&](uint32_t at) {     // of the four from `at` on, as bits
+    uint32_t bits = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      if (at + i < p.pages && p.refs[at + i] == 0) bits |= 1u << i;
+    return bits;
+  };
+  const uint32_t free_first = free_pages(4 * threadIdx.x);
+  int bad = slots_valid(p, sm + p.batch, slot, first) ? 0 : (int)kFlagSlot;
   // sequences [b0, b1) are this thread's: ranks follow the sequence order
   const uint32_t per = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS;
   const uint32_t b0 = min(p.batch, threadIdx.x * per), b1 = min(p.batch, b0 + per);
@@ -132,11 +144,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
   // the first `total` free pages, lowest first
   uint32_t found = 0;
   for (uint32_t base = 0; base < p.pages && found < total; base += 4 * PLAN_THREADS) {
-    uint32_t mine = 0;
-    const uint32_t at = base + 4 * threadIdx.x;
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-      if (at + i < p.pages && p.refs[at + i] == 0) mine |= 1u << i;
+    const uint32_t at = base + 4 * threadIdx.x, mine = base ? free_pages(at) : free_first;
     uint32_t n;
     uint32_t r = found + block_scan(__popc(mine), &n);
 #pragma unroll
@@ -174,9 +182,8 @@ struct ForkParams {
   const int32_t* parent;
   int32_t* slot_out;
   int32_t advance_by;
-  // scratch: free slots [slots]; touched slots, where each copies from (-1: it is only
-  // emptied) and its rows [2 batch]; how many are copies, how many there are
-  int32_t* free_list;
+  // scratch: touched slots, where each copies from (-1: it is only emptied) and its rows
+  // [2 batch]; how many are copies, how many there are
   int32_t* dst;
   int32_t* src;
   int32_t* rows;
@@ -185,8 +192,12 @@ struct ForkParams {
   uint32_t layers, heads;
 };
 
-// Shared memory: the slots, the parents, the eldest child of every sequence, and
-// bitmaps over all slots: "named by slot[]" and "kept".
+// Shared memory: the slots, the parents, the eldest child of every sequence, its rows, the
+// free slots that are taken, and bitmaps over all slots: "named by slot[]", "kept" and "holds
+// no rows".  Global memory is asked three times: for what the call names and the slots' row
+// counts, for the named ones' counts, and to write.
+uint32_t fork_plan_smem(uint32_t batch, uint32_t slots) { return 5 * batch * 4 + 3 * ((slots + 31) / 32) * 4; }
+
 __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const ForkParams f) {
   extern __shared__ uint32_t sm[];
   __shared__ uint32_t emptied;
@@ -195,24 +206,34 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const Fo
   int32_t* slot = reinterpret_cast<int32_t*>(sm);
   int32_t* parent = slot + p.batch;
   uint32_t* eldest = sm + 2 * p.batch;
-  uint32_t* named = eldest + p.batch;
+  int32_t* rows = reinterpret_cast<int32_t*>(sm + 3 * p.batch);
+  int32_t* taken = reinterpret_cast<int32_t*>(sm + 4 * p.batch);
+  uint32_t* named = sm + 5 * p.batch;
   uint32_t* kept = named + words;
+  uint32_t* none = kept + words;
   pdl_wait();
   pdl_launch_dependents();
+  const int32_t first_slot = tid < p.batch ? p.slot[tid] : -1;
+  const int32_t first_parent = tid < p.batch ? f.parent[tid] : -1;
   int bad = 0;
+  for (uint32_t s = tid; s < words * 32; s += PLAN_THREADS) {      // whole warps
+    const uint32_t w = __ballot_sync(0xffffffffu, s < p.slots && p.tokens[s] == 0);
+    if (s % 32 == 0) none[s / 32] = w;
+  }
   for (uint32_t i = tid; i < words; i += PLAN_THREADS) kept[i] = 0;
   for (uint32_t b = tid; b < p.batch; b += PLAN_THREADS) {
     eldest[b] = 0xffffffffu;
-    parent[b] = f.parent[b];
+    parent[b] = b == tid ? first_parent : f.parent[b];
     if (parent[b] < -1 || parent[b] >= (int32_t)p.batch) bad |= kFlagSlot;
   }
   if (tid == 0) emptied = 0;
-  if (!slots_valid(p, named, slot)) bad |= kFlagSlot;
+  if (!slots_valid(p, named, slot, first_slot)) bad |= kFlagSlot;
   if (!bad)
     for (uint32_t b = tid; b < p.batch; b += PLAN_THREADS) {
       if (slot[b] < 0) continue;
       const int64_t n = p.tokens[slot[b]];
       if (n < 0 || !rows_fit(n + f.advance_by, p.max_pages)) bad |= kFlagCacheRow;
+      rows[b] = (int32_t)(n + f.advance_by);
     }
   if (__syncthreads_or(bad)) {           // nothing is changed
     if (tid == 0) f.counts[0] = f.counts[1] = 0;
@@ -222,7 +243,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const Fo
   }
   auto source = [&](uint32_t b) { return parent[b] >= 0 ? slot[parent[b]] : -1; };
   for (uint32_t b = tid; b < p.batch; b += PLAN_THREADS) {
-    if (f.advance_by && slot[b] >= 0) p.tokens[slot[b]] += f.advance_by;
+    if (f.advance_by && slot[b] >= 0) p.tokens[slot[b]] = rows[b];
     const int32_t s = source(b);
     if (s >= 0) {
       atomicMin(eldest + parent[b], b);
@@ -239,7 +260,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const Fo
   auto is_free = [&](uint32_t s) {
     const uint32_t bit = 1u << (s & 31);
     if (kept[s >> 5] & bit) return false;
-    return (named[s >> 5] & bit) != 0 || p.tokens[s] == 0;
+    return ((named[s >> 5] | none[s >> 5]) & bit) != 0;
   };
   const uint32_t per = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS;
   const uint32_t b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
@@ -254,7 +275,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const Fo
   uint32_t r = before & 0x1ffff;
   for (uint32_t s = s0; s < s1; ++s)
     if (is_free(s)) {
-      f.free_list[r] = s;
+      if (r < given) taken[r] = s;
       if (r >= given && (named[s >> 5] >> (s & 31) & 1u)) {     // given up and not taken
         const uint32_t e = given + atomicAdd(&emptied, 1);
         f.dst[e] = s;
@@ -271,10 +292,10 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const Fo
       const int32_t from = to;
       to = -1;
       if (rank < given) {
-        to = f.free_list[rank];
+        to = taken[rank];
         f.dst[rank] = to;
         f.src[rank] = from;
-        f.rows[rank] = p.tokens[from];
+        f.rows[rank] = rows[parent[b]];
       }
       ++rank;
     }
@@ -287,8 +308,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_fork_plan_kernel(const Fo
   }
 }
 
-// A warp copies the open rows of one (copy, layer, K or V, head), up to 8 KB, four loads a lane
-// at a time: 9 us of the 19 above, a copy's rate while it runs and latency around it.  A block does the
+// A warp copies the open rows of one (copy, layer, K or V, head), up to 8 KB, eight loads a
+// lane at a time (64 x 4 beams: 17.7 us, with four 18.3, with sixteen 18.4); a block does the
 // table row, count and page references of one touched slot.  A source slot is a
 // kept one and a destination is not, so nothing is read that another one writes.
 __global__ void __launch_bounds__(COPY_THREADS) kv8_fork_copy_kernel(const ForkParams f) {
@@ -319,13 +340,13 @@ __global__ void __launch_bounds__(COPY_THREADS) kv8_fork_copy_kernel(const ForkP
     const size_t layer = (size_t)l * p.slots;
     const uint4* from = reinterpret_cast<const uint4*>(f.tails + ((layer + src) * parts + kvh) * BLOCK_CODES);
     uint4* to = reinterpret_cast<uint4*>(f.tails + ((layer + dst) * parts + kvh) * BLOCK_CODES);
-    for (uint32_t e = lane; e < n; e += 4 * 32) {
-      uint4 x[4];
+    for (uint32_t e = lane; e < n; e += 8 * 32) {
+      uint4 x[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 8; ++k)
         if (e + 32 * k < n) x[k] = from[e + 32 * k];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 8; ++k)
         if (e + 32 * k < n) to[e + 32 * k] = x[k];
     }
   }
@@ -560,11 +581,14 @@ int kv8_fork_launch(const pvlc_kv8_cache& c, const int32_t* slot, const int32_t*
   f.dst = s + 4;
   f.src = f.dst + 2 * batch;
   f.rows = f.src + 2 * batch;
-  f.free_list = f.rows + 2 * batch;
   f.tails = reinterpret_cast<__half*>(c.tails);
   f.layers = c.layers;
   f.heads = c.kv_heads;
-  const uint32_t smem = 3 * batch * 4 + 2 * ((c.slots + 31) / 32) * 4;
+  const uint32_t smem = kv8::fork_plan_smem(batch, c.slots);
+  if (const int st = set_smem_attribute_once(
+          reinterpret_cast<const void*>(kv8::kv8_fork_plan_kernel),
+          kv8::fork_plan_smem(PVLC_KV8_MAX_BATCH, PVLC_KV8_MAX_SLOTS)))
+    return st;
   if (const int st = launch(kv8::kv8_fork_plan_kernel, f, dim3(1), kv8::PLAN_THREADS, smem, stream))
     return st;
   // a warp for each copy where all but one sequence move, up to eight blocks an SM
