@@ -220,21 +220,23 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) beam_chunk_kernel(const Param
     listed = LIST + 1;                       // fewer than K groups hold anything
   }
   __syncthreads();
-  if (tid == 0) {
-    float2 all = warp_sum[0];
+  // the last warp joins the sums while the first ones rank: both chains are long
+  if (warp == THREADS / 32 - 1) {
+    const float2 x = lane < THREADS / 32 ? warp_sum[lane] : make_float2(-CUDART_INF_F, 0.f);
+    float top = x.x;
 #pragma unroll
-    for (int i = 1; i < THREADS / 32; ++i) all.x = fmaxf(all.x, warp_sum[i].x);
-    all.y = 0.f;
+    for (int o = THREADS / 64; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float all = x.x > -CUDART_INF_F ? x.y * fast_exp2((x.x - top) * kLog2e) : 0.f;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i)
-      if (warp_sum[i].x > -CUDART_INF_F) all.y += warp_sum[i].y * fast_exp2((warp_sum[i].x - all.x) * kLog2e);
-    p.sums[slot] = all;
+    for (int o = THREADS / 64; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) p.sums[slot] = make_float2(top, all);
   }
   const uint32_t n = listed;
   if (n <= LIST) {
     for (uint32_t i = tid; i < n; i += THREADS) {
       const u64 mine = list[i];
       uint32_t rank = 0;
+#pragma unroll 8
       for (uint32_t j = 0; j < n; ++j) rank += list[j] > mine;
       if (rank < K) keys[rank] = mine;
     }
@@ -276,7 +278,9 @@ __device__ __forceinline__ Cand shfl(const Cand& c, int o) {
 __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
   __shared__ double base[PVLC_BEAM_MAX_BEAMS];
   __shared__ Cand part[THREADS / 32];
-  __shared__ Cand list[LIST];
+  __shared__ double list_score[LIST];
+  __shared__ u64 list_key[LIST];
+  __shared__ uint32_t list_beam[LIST];
   __shared__ __align__(16) float head_score[MAX_HEADS];
   __shared__ float bound_out;
   __shared__ uint32_t listed;
@@ -352,7 +356,11 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
       auto add = [&](const Cand& c) {        // a chunk's list is in order: false behind the last
         if (c.key == 0 || c.score < (double)bound) return false;
         const uint32_t at = atomicAdd(&listed, 1);
-        if (at < LIST) list[at] = c;
+        if (at < LIST) {
+          list_score[at] = c.score;
+          list_key[at] = c.key;
+          list_beam[at] = c.beam;
+        }
         return true;
       };
       bool more = true;
@@ -364,9 +372,14 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
     const uint32_t found = listed;
     if (found <= LIST) {
       for (uint32_t i = threadIdx.x; i < found; i += THREADS) {
-        const Cand c = list[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < found; ++j) rank += before(list[j], c);
+        const Cand c{list_score[i], list_beam[i], list_key[i]};
+        uint32_t rank = 0;                   // how many are before() it
+#pragma unroll 4
+        for (uint32_t j = 0; j < found; ++j) {
+          const bool same = list_score[j] == c.score, beam = list_beam[j] == c.beam;
+          rank += (list_score[j] > c.score) |
+                  (same & ((list_beam[j] < c.beam) | (beam & (list_key[j] > c.key))));
+        }
         if (rank < K) write(rank, c);
       }
       return;
