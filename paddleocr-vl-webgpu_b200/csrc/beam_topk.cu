@@ -22,12 +22,15 @@
 // Keys are unique, so nothing depends on the order in which threads arrive.
 //
 // Measured, calls back to back, a vocabulary of 103,424, the best 8:
-//   64 x 4 beams, f32, 106 MB   26.7 us   4.0 TB/s, 60 % of a copy; the chunks take 20 of
-//     them, the join the rest: one block a request, bound by the latency of its chain of
-//     sums, logarithm and ranking
-//   1 x 4 beams, fp16   7.5 us   two launches' latency
+//   64 x 4 beams, f32, 106 MB   25.4 us   4.2 TB/s, 64 % of a copy: 16.4 for the loads,
+//     maxima and exponentials alone (a copy's rate), 0.8 for the bound, 4.1 for listing and
+//     ranking, 4.1 for the join, one block a request, which is bound by the latency of its
+//     chain of sums, logarithm and ranking
+//   1 x 4 beams, fp16   6.6 us   two launches' latency
 // A join by the block that leaves a request's last chunk, in one launch, took 38.9 us against 27.9:
 // each block then holds its place on the SM for a fence and an atomic's way there and back.
+// Blocks that go from chunk to chunk with the next one's loads under the ranking took 34.3
+// (five an SM, whose registers then spill) and 30.4 (four).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
