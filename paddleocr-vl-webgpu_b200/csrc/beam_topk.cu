@@ -16,9 +16,10 @@
 //
 // Selection: of any disjoint groups' maxima the K-th largest is a bound that at
 // least K elements reach, so only what reaches it is looked at -- in a chunk, of
-// the maxima of 64 groups of 4 lanes; in a join, of the chunks' best -- a few
-// dozen elements, which are ranked by counting.  Where too many reach the bound
-// (equal or masked logits) the K are taken one at a time.
+// the maxima of 64 groups of 4 lanes; in a join, of the chunks' best, or of the
+// first few of each where there are not K chunks -- a few
+// dozen elements, which are ranked by counting.  Where too many reach the bound (equal
+// logits) the K are taken one at a time.
 // Keys are unique, so nothing depends on the order in which threads arrive.
 //
 // Measured, calls back to back, a vocabulary of 103,424, the best 8:
@@ -45,7 +46,7 @@ namespace beam {
 
 constexpr int THREADS = 256;
 constexpr uint32_t LIST = 512;               // elements ranked by counting
-constexpr uint32_t MAX_HEADS = 2 * THREADS;  // chunks of a request that a join bounds by
+constexpr uint32_t MAX_HEADS = 2 * THREADS;  // elements of a request that a join bounds by
 constexpr int BLOCKS = 5;                    // of an SM: 27.8 us for the 64 x 4 beams, 29.2 with 4
 
 typedef unsigned long long u64;
@@ -198,29 +199,25 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) beam_chunk_kernel(const Param
   u64* keys = p.keys + slot * K;
   const float bound = kth_largest(group_top, GROUPS, K, &bound_out);
   auto key_of = [](float y, uint32_t at) -> u64 { return (u64)ordered(y) << 32 | (0xffffffffu - at); };
-  if (bound > -CUDART_INF_F) {
-    // The warp looks at each thread that has something together, one of its logits a lane,
-    // handed over through shared memory: as unrolled code on registers this rare work took
-    // longer to fetch than to run.
-    uint32_t found = __ballot_sync(0xffffffffu, best >= bound);
-    while (found) {
-      const uint32_t who = __ffs(found) - 1;
-      found &= found - 1;
-      if (lane == who) {
+  // The warp looks at each thread that has something together, one of its logits a lane,
+  // handed over through shared memory: as unrolled code on registers this rare work took
+  // longer to fetch than to run.  Masked logits are left to the end.
+  uint32_t found = __ballot_sync(0xffffffffu, best >= bound && best > -CUDART_INF_F);
+  while (found) {
+    const uint32_t who = __ffs(found) - 1;
+    found &= found - 1;
+    if (lane == who) {
 #pragma unroll
-        for (int i = 0; i < PER; i += 4)
-          *reinterpret_cast<float4*>(handed[warp] + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-      }
-      __syncwarp();
-      const float y = lane < PER ? handed[warp][lane] : -CUDART_INF_F;
-      if (y >= bound) {
-        const uint32_t to = atomicAdd(&listed, 1);
-        if (to < LIST) list[to] = key_of(y, token(warp * 32 + who, lane));
-      }
-      __syncwarp();
+      for (int i = 0; i < PER; i += 4)
+        *reinterpret_cast<float4*>(handed[warp] + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
-  } else if (tid == 0) {
-    listed = LIST + 1;                       // fewer than K groups hold anything
+    __syncwarp();
+    const float y = lane < PER ? handed[warp][lane] : -CUDART_INF_F;
+    if (y >= bound && y > -CUDART_INF_F) {
+      const uint32_t to = atomicAdd(&listed, 1);
+      if (to < LIST) list[to] = key_of(y, token(warp * 32 + who, lane));
+    }
+    __syncwarp();
   }
   __syncthreads();
   // the last warp joins the sums while the first ones rank: both chains are long
@@ -242,6 +239,18 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) beam_chunk_kernel(const Param
 #pragma unroll 8
       for (uint32_t j = 0; j < n; ++j) rank += list[j] > mine;
       if (rank < K) keys[rank] = mine;
+    }
+    if (n < K && warp == 0) {                // then the first masked ones, then none
+      uint32_t have = n;
+      const uint32_t end = min(p.vocab, (c + 1) * CHUNK);
+      for (uint32_t at = c * CHUNK + lane; have < K && at - lane < end; at += 32) {
+        const bool masked = at < end && !(to_float(x[at]) > -CUDART_INF_F);
+        const uint32_t all = __ballot_sync(0xffffffffu, masked);
+        const uint32_t rank = have + __popc(all & ((1u << lane) - 1));
+        if (masked && rank < K) keys[rank] = key_of(-CUDART_INF_F, at);
+        have += __popc(all);
+      }
+      for (uint32_t k = have + lane; k < K; k += 32) keys[k] = 0;
     }
     return;
   }
@@ -289,13 +298,16 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
   __shared__ uint32_t listed;
   const uint32_t r = blockIdx.x, W = p.beams, K = p.topk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t per = p.chunks * K, heads = W * p.chunks, n = W * per;
+  // the first `each` of every chunk bound the rest: at least K of them
+  const uint32_t per = p.chunks * K, chunks = W * p.chunks, n = W * per;
+  const uint32_t each = chunks < K ? (K + chunks - 1) / chunks : 1, heads = chunks * each;
   const u64* keys = p.keys + (size_t)r * n;
-  const bool bounded = heads >= K && heads <= MAX_HEADS;
+  const bool bounded = heads <= MAX_HEADS;
+  auto chunk_of = [&](uint32_t i) { return each == 1 ? i : i / each; };
   if (threadIdx.x == 0) listed = 0;
   pdl_wait();
   pdl_launch_dependents();
-  // this thread's chunks' first keys, in flight under the log-sums
+  // this thread's first keys and what follows them, in flight under the log-sums
   constexpr uint32_t EARLY = 2;
   u64 mine[2][EARLY];
 #pragma unroll
@@ -303,7 +315,8 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
 #pragma unroll
     for (uint32_t k = 0; k < EARLY; ++k) {
       const uint32_t i = threadIdx.x + e * THREADS;
-      mine[e][k] = bounded && i < heads && k < K ? keys[(size_t)i * K + k] : 0;
+      const uint32_t chunk = chunk_of(i), at = i - chunk * each + k;
+      mine[e][k] = bounded && i < heads && at < K ? keys[(size_t)chunk * K + at] : 0;
     }
   for (uint32_t w = warp; w < W; w += THREADS / 32) {
     const float2* s = p.sums + (size_t)(r * W + w) * p.chunks;
@@ -342,12 +355,12 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
     p.out_token[at] = (int32_t)(0xffffffffu - (uint32_t)c.key);
   };
   if (bounded) {
-    // scores rounded down to f32: at least K chunks' best reach the K-th largest of them
+    // scores rounded down to f32: at least K of the first ones reach the K-th largest of them
     float score[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t i = threadIdx.x + e * THREADS;
-      score[e] = i < heads ? __double2float_rd(made(mine[e][0], i / p.chunks).score) : -CUDART_INF_F;
+      score[e] = i < heads ? __double2float_rd(made(mine[e][0], chunk_of(i) / p.chunks).score) : -CUDART_INF_F;
       head_score[i] = score[e];
     }
     __syncthreads();
@@ -366,10 +379,11 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
         }
         return true;
       };
-      bool more = true;
+      const uint32_t chunk = chunk_of(i), at = i - chunk * each, beam = chunk / p.chunks;
+      bool more = add(made(mine[e][0], beam)) && at == each - 1;      // the last of them goes on
 #pragma unroll
-      for (uint32_t k = 0; k < EARLY; ++k) more = more && add(made(mine[e][k], i / p.chunks));
-      for (uint32_t k = EARLY; k < K && more; ++k) more = add(candidate(i * K + k));
+      for (uint32_t k = 1; k < EARLY; ++k) more = more && add(made(mine[e][k], beam));
+      for (uint32_t k = at + EARLY; k < K && more; ++k) more = add(candidate(chunk * K + k));
     }
     __syncthreads();
     const uint32_t found = listed;

@@ -198,3 +198,28 @@ def test_wrapper_refusals(cuda_lib):
         ops.beam_topk(x, s, 8, ops.BeamWorkspace(1, 1, 100, 1))
     with pytest.raises(ValueError):
         ops.beam_topk(x, s, 4, out=(s, s.int(), s.int()[:1]))
+
+
+@pytest.mark.parametrize("B,W,V,K", [(1, 1, 40, 16), (2, 4, 150, 16), (2, 2, 4097, 24), (1, 3, 8193, 64),
+                                     (40, 4, 9000, 12)])
+@pytest.mark.parametrize("left", [0, 1, 5, 12, 30])
+def test_few_tokens_allowed(cuda_lib, B, W, V, K, left):
+    """A mask that leaves `left` tokens of a row, first and last ones among them, and other rows
+    with a NaN for each masked one: fewer than K continuations are finite, or just as many."""
+    rng = np.random.default_rng(left * 7 + V)
+    x = np.full((B * W, V), -np.inf, np.float32)
+    for r in range(B * W):
+        at = rng.choice(V, left, replace=False)
+        if left > 1:
+            at[:2] = 0, V - 1
+        if r % 3 == 1:
+            x[r] = np.nan
+        x[r, at] = rng.standard_normal(left) * 3
+    check(x, (-5 * rng.random((B, W))).astype(np.float32), K)
+
+
+@pytest.mark.parametrize("B,W,V,K", [(3, 1, 5000, 64), (2, 2, 300, 33), (1, 8, 70, 48), (7, 5, 2000, 17)])
+def test_more_wanted_than_there_are_chunks(cuda_lib, B, W, V, K):
+    rng = np.random.default_rng(K)
+    check((rng.standard_normal((B * W, V)) * 3).astype(np.float32),
+          (-2 * rng.random((B, W))).astype(np.float32), K)
