@@ -429,8 +429,8 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Params p) {
 }
 
 // Logits a thread.  A chunk costs about 2 us beside its loads, so 32, as many as the registers
-// of five blocks an SM hold: 64 x 4 beams take 27.6 us, with 16 and seven blocks 32.1, with 8
-// 67.9; 4 x 4 beams 8.7, 9.1, 15.3.  Where such chunks would leave half the SMs without one, 16:
+// of five blocks an SM hold: 64 x 4 beams took 27.6 us, with 16 and seven blocks 32.1, with 8
+// 67.9, when all were tried; 4 x 4 beams 8.7, 9.1, 15.3.  Where such chunks would leave half the SMs without one, 16:
 // one row takes 6.4 us against 7.7, 1 x 4 beams 7.2 against 7.6, but 2 x 4 beams 8.2 against 7.7.
 uint32_t per_thread(uint32_t rows, uint32_t vocab) {
   const uint64_t wide = (vocab + THREADS * 32 - 1) / (THREADS * 32);
