@@ -18,11 +18,11 @@
 // group of 8.  That is 6 % of the tensor cores' rate, so mma.sync on registers,
 // which needs no second copy of the codes, is enough (their pipe is active 15 % of
 // the time).  Measured, a layer of 16 query and 2 KV heads, calls back to back:
-//   64 sequences of 606 .. 8,011 rows   34.3 us   4.3 TB/s, 65 % of a copy
+//   64 sequences of 606 .. 8,011 rows   34.2 us   4.3 TB/s, 65 % of a copy
 //   16 sequences, 8 KV heads, 4 k .. 8 k rows   37.9 us   4.8 TB/s, 72 %
-//   64 x 4 beams of 1,248 .. 1,499 rows   44.9 us   190 MB through L2, 55 MB of them distinct
-//   1 sequence of 1,023 rows   9.9 us   bound by its chain of dependent loads
-// Of the 34.3 us 22.3 are the stream at a copy's rate.  4 pass before the first
+//   64 x 4 beams of 1,248 .. 1,499 rows   44.4 us   190 MB through L2, 55 MB of them distinct
+//   1 sequence of 1,023 rows   9.5 us   bound by its chain of dependent loads
+// Of the 34.2 us 22.3 are the stream at a copy's rate.  4 pass before the first
 // page lands (launch, the sequences' slots, lengths and page ids, each read after
 // the other), 3 in joining the split units, the rest in the uneven end: without
 // its arithmetic the kernel takes 32.3, without its pages 29.4.  The beams are
@@ -126,48 +126,50 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& pair, uint32_
   rest = pack_half2(a - h.x, b - h.y);
 }
 
-// 16 dims d .. d + 15 (d a multiple of 16, below 64) and their partners 64
-// above, rotated: lo cos - hi sin, hi cos + lo sin; as fp16 pairs.  SPLIT: and what
-// those round off; returns the 32 values' sum.
-template <bool SPLIT>
-__device__ __forceinline__ float rotate16(const __half* row, uint32_t d, const DecodeParams& p,
-                                          uint32_t r, uint32_t* lo_out, uint32_t* hi_out,
-                                          uint32_t* lo_rest, uint32_t* hi_rest) {
-  float sum = 0.f;
+// The rotation of 16 dims d .. d + 15 (d a multiple of 16, below 64) of a row and their
+// partners 64 above: lo cos - hi sin, hi cos + lo sin.
+struct Turns {                        // the table's values
+  float4 cl[4], ch[4], sl[4], sh[4];
+  __device__ __forceinline__ Turns(const DecodeParams& p, uint32_t d, uint32_t r) {
 #pragma unroll
-  for (int e = 0; e < 16; e += 4) {
-    const uint2 lw = __ldg(reinterpret_cast<const uint2*>(row + d + e));
-    const uint2 hw = __ldg(reinterpret_cast<const uint2*>(row + d + 64 + e));
-    const size_t at = ((size_t)mrope_axis(d + e) * p.rope_rows + r) * HD + d + e;
-    const float4 cl = __ldg(reinterpret_cast<const float4*>(p.rope_cos + at));
-    const float4 ch = __ldg(reinterpret_cast<const float4*>(p.rope_cos + at + 64));
-    const float4 sl = __ldg(reinterpret_cast<const float4*>(p.rope_sin + at));
-    const float4 sh = __ldg(reinterpret_cast<const float4*>(p.rope_sin + at + 64));
-    const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&lw.x));
-    const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&lw.y));
-    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hw.x));
-    const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hw.y));
+    for (int e = 0; e < 4; ++e) {
+      const size_t at = ((size_t)mrope_axis(d + 4 * e) * p.rope_rows + r) * HD + d + 4 * e;
+      cl[e] = __ldg(reinterpret_cast<const float4*>(p.rope_cos + at));
+      ch[e] = __ldg(reinterpret_cast<const float4*>(p.rope_cos + at + 64));
+      sl[e] = __ldg(reinterpret_cast<const float4*>(p.rope_sin + at));
+      sh[e] = __ldg(reinterpret_cast<const float4*>(p.rope_sin + at + 64));
+    }
+  }
+};
+struct Piece {                        // a row's values
+  uint2 lo[4], hi[4];
+  __device__ __forceinline__ Piece(const __half* row, uint32_t d) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo[e] = __ldg(reinterpret_cast<const uint2*>(row + d + 4 * e));
+      hi[e] = __ldg(reinterpret_cast<const uint2*>(row + d + 64 + 4 * e));
+    }
+  }
+  // put(i, x, y): pair i of the low dims, 8 + i of the high ones
+  template <typename F>
+  __device__ __forceinline__ void rotate(const Turns& t, F put) const {
     auto turn = [](float x, float c, float y, float s) {
       return __fadd_rn(__fmul_rn(x, c), __fmul_rn(y, s));
     };
-    const int w = e / 2;
-    auto put = [&](float a, float b, uint32_t* out, uint32_t* rest) {
-      if (SPLIT) {
-        split2(a, b, *out, *rest);
-        sum += a + b;
-      } else {
-        *out = pack_half2(a, b);
-      }
-    };
-    put(turn(l0.x, cl.x, -h0.x, sl.x), turn(l0.y, cl.y, -h0.y, sl.y), lo_out + w, lo_rest + w);
-    put(turn(l1.x, cl.z, -h1.x, sl.z), turn(l1.y, cl.w, -h1.y, sl.w), lo_out + w + 1,
-        lo_rest + w + 1);
-    put(turn(h0.x, ch.x, l0.x, sh.x), turn(h0.y, ch.y, l0.y, sh.y), hi_out + w, hi_rest + w);
-    put(turn(h1.x, ch.z, l1.x, sh.z), turn(h1.y, ch.w, l1.y, sh.w), hi_out + w + 1,
-        hi_rest + w + 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&lo[e].x));
+      const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&lo[e].y));
+      const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[e].x));
+      const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[e].y));
+      const float4 &c = t.cl[e], &d = t.ch[e], &s = t.sl[e], &u = t.sh[e];
+      put(2 * e, turn(l0.x, c.x, -h0.x, s.x), turn(l0.y, c.y, -h0.y, s.y));
+      put(2 * e + 1, turn(l1.x, c.z, -h1.x, s.z), turn(l1.y, c.w, -h1.y, s.w));
+      put(2 * e + 8, turn(h0.x, d.x, l0.x, u.x), turn(h0.y, d.y, l0.y, u.y));
+      put(2 * e + 9, turn(h1.x, d.z, l1.x, u.z), turn(h1.y, d.w, l1.y, u.w));
+    }
   }
-  return sum;
-}
+};
 
 // The low / high two code bytes of a word as an fp16 pair (exact).
 template <int CODE>
@@ -810,14 +812,24 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         return;
       }
       uint8_t* slot = slots + s * seq_slot<NT>();
+      // The new rows' loads go with q's, and the key takes the same table values: 1 x 1,023 rows
+      // 9.8 -> 9.5 us, 169 sequences of 22 .. 57 rows with 8 KV heads 43.8 -> 41.9.
+      const size_t new_row = (size_t)it.b * p.kv_stride + it.h * HD;
+      const uint32_t d = 16 * (lane & 3);
+      const Turns turns(p, d, it.sq.rope);
+      const Piece key(p.k_new + new_row, d);
+      const uint4 value = __ldg(reinterpret_cast<const uint4*>(p.v_new + new_row) + (lane & 15));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         uint32_t w[16], rest[16];
         const uint32_t head = nt * 8 + (lane >> 2);
         float sum = 0.f;
         if (head < G) {
-          sum = rotate16<true>(p.q + (size_t)it.b * p.q_stride + ((size_t)it.h * G + head) * HD,
-                               16 * (lane & 3), p, it.sq.rope, w, w + 8, rest, rest + 8);
+          const Piece q(p.q + (size_t)it.b * p.q_stride + ((size_t)it.h * G + head) * HD, d);
+          q.rotate(turns, [&](int i, float x, float y) {
+            split2(x, y, w[i], rest[i]);
+            sum += x + y;
+          });
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) w[e] = rest[e] = 0;
@@ -838,22 +850,19 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         uint4* kn = reinterpret_cast<uint4*>(slot + 2 * NT * 2048);
         uint4* vn = kn + 16;
         if (lane < 4) {
-          uint32_t w[16];
-          rotate16<false>(p.k_new + (size_t)it.b * p.kv_stride + it.h * HD, 16 * lane, p,
-                          it.sq.rope, w, w + 8, nullptr, nullptr);
+          uint32_t kw[16];
+          key.rotate(turns, [&](int i, float x, float y) { kw[i] = pack_half2(x, y); });
           uint4* row = reinterpret_cast<uint4*>(tail_rows(p.c, it.sq.slot, 0, it.h) + last * HD);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint4 x = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+            const uint4 x = make_uint4(kw[4 * e], kw[4 * e + 1], kw[4 * e + 2], kw[4 * e + 3]);
             const int at = (e & 2) * 4 + 2 * lane + (e & 1);
             row[at] = x;
             kn[at] = x;
           }
         } else if (lane >= 16) {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(
-                                    p.v_new + (size_t)it.b * p.kv_stride + it.h * HD) + lane - 16);
-          reinterpret_cast<uint4*>(tail_rows(p.c, it.sq.slot, 1, it.h) + last * HD)[lane - 16] = x;
-          vn[lane - 16] = x;
+          reinterpret_cast<uint4*>(tail_rows(p.c, it.sq.slot, 1, it.h) + last * HD)[lane - 16] = value;
+          vn[lane - 16] = value;
         }
         __syncwarp();
       }
