@@ -195,18 +195,9 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1152.f));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Key codes: int8 ones with 1152 added, which costs no instruction to leave in and is taken
-// off the score as 1152 times the sum of q.  (Not so for values, whose sum over the rows cancels.)
-constexpr float KEY_BIAS = 1152.f;
-template <int CODE>
-__device__ __forceinline__ uint32_t key_lo(uint32_t w) {
-  return CODE == PVLC_KV8_E4M3 ? codes_lo<CODE>(w) : __byte_perm(w, 0x64646464u, 0x4140);
-}
-template <int CODE>
-__device__ __forceinline__ uint32_t key_hi(uint32_t w) {
-  return CODE == PVLC_KV8_E4M3 ? codes_hi<CODE>(w) : __byte_perm(w, 0x64646464u, 0x4342);
-}
-// A loaded word of codes as codes_lo / codes_hi take it.
+// A loaded word of codes as codes_lo / codes_hi take it.  (int8 keys that keep their 1152 until the
+// score is made save a subtraction an operand word, but the sums then hold 1152 sum(q) beside the
+// score, and lose up to ten of its bits where the q of a head have a common part.)
 template <int CODE>
 __device__ __forceinline__ uint32_t biased(uint32_t w) {
   return CODE == PVLC_KV8_E4M3 ? w : w ^ 0x80808080u;
@@ -225,7 +216,7 @@ struct Acc {
 // eight above) into weights, with the running maximum; `live` keys count.
 template <int NT>
 __device__ __forceinline__ void weigh(float (&s)[2][NT][4], Acc<NT>& a, float kk,
-                                      const float (&off)[NT][2], float rsv, int key0, int live, uint32_t (&w)[2][NT][2]) {
+                                      float off, float rsv, int key0, int live, uint32_t (&w)[2][NT][2]) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float t0 = -CUDART_INF_F, t1 = -CUDART_INF_F;
@@ -235,8 +226,8 @@ __device__ __forceinline__ void weigh(float (&s)[2][NT][4], Acc<NT>& a, float kk
       for (int r = 0; r < 2; ++r) {
         float* x = s[mt][nt] + 2 * r;
         const bool on = key0 + 16 * mt + 8 * r < live;
-        x[0] = on ? x[0] * kk + off[nt][0] : -CUDART_INF_F;
-        x[1] = on ? x[1] * kk + off[nt][1] : -CUDART_INF_F;
+        x[0] = on ? x[0] * kk + off : -CUDART_INF_F;
+        x[1] = on ? x[1] * kk + off : -CUDART_INF_F;
         t0 = fmaxf(t0, x[0]);
         t1 = fmaxf(t1, x[1]);
       }
@@ -282,7 +273,7 @@ __device__ __forceinline__ uint4 rest_words(const uint8_t* rest, int nt, int i) 
 template <int CODE, int NT>
 __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv, float qk,
                                           const uint32_t (&qf)[NT][16], const uint8_t* rest,
-                                          const float* bias, Acc<NT>& a, int g, int t) {
+                                          Acc<NT>& a, int g, int t) {
   const int pi = (g >> 1) | ((g & 1) << 2);
   float s[2][NT][4], low[2][NT][4];
 #pragma unroll
@@ -313,8 +304,8 @@ __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv,
         for (int mt = 0; mt < 2; ++mt) {
           const int i = 2 * f + e;
           const uint32_t ya = biased<CODE>(wa[mt][i]), yb = biased<CODE>(wb[mt][i]);
-          const uint32_t a0 = key_lo<CODE>(ya), a1 = key_lo<CODE>(yb);
-          const uint32_t a2 = key_hi<CODE>(ya), a3 = key_hi<CODE>(yb);
+          const uint32_t a0 = codes_lo<CODE>(ya), a1 = codes_lo<CODE>(yb);
+          const uint32_t a2 = codes_hi<CODE>(ya), a3 = codes_hi<CODE>(yb);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_16816(s[mt][nt], a0, a1, a2, a3, qf[nt][8 * j + 2 * i], qf[nt][8 * j + 2 * i + 1]);
@@ -330,15 +321,8 @@ __device__ __forceinline__ void page_tile(const uint8_t* st, float sk, float sv,
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[mt][nt][e] += low[mt][nt][e];
   uint32_t w[2][NT][2];
-  // t = s kk + log2(scale_V), less the keys' bias
-  const float kk = sk * qk, lsv = __log2f(sv);
-  float off[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      off[nt][c] = CODE == PVLC_KV8_E4M3 ? lsv : lsv - bias[nt * 8 + 2 * t + c] * kk;
-  weigh<NT>(s, a, kk, off, __frcp_rn(sv), 0, 64, w);
+  // t = s kk + log2(scale_V)
+  weigh<NT>(s, a, sk * qk, __log2f(sv), __frcp_rn(sv), 0, 64, w);
   // value rows t, t + 4, t + 8, t + 12 of a half tile: keys pi(2 t), pi(2 t + 1), ..
   const uint8_t* v = st + 4096;
 #pragma unroll
@@ -402,8 +386,7 @@ __device__ __forceinline__ void tail_tile(const uint8_t* kt, const uint8_t* vt, 
       }
   }
   uint32_t w[2][NT][2];
-  const float off[NT][2] = {};
-  weigh<NT>(s, a, qk, off, 1.f, pi, last + 1, w);
+  weigh<NT>(s, a, qk, 0.f, 1.f, pi, last + 1, w);
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -600,9 +583,9 @@ struct Units {
 };
 
 // A unit's rotated q as the consumers' fragments [NT][4][32 lanes] x 16 bytes, what it rounds
-// off in the same form, then its new key and value rows and each head's key bias (16 floats).
+// off in the same form, then its new key and value rows.
 template <int NT>
-constexpr uint32_t seq_slot() { return 2 * NT * 2048 + 512 + 64; }
+constexpr uint32_t seq_slot() { return 2 * NT * 2048 + 512; }
 
 template <int NT>
 constexpr uint32_t fixed_smem() {
@@ -823,20 +806,13 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
       for (int nt = 0; nt < NT; ++nt) {
         uint32_t w[16], rest[16];
         const uint32_t head = nt * 8 + (lane >> 2);
-        float sum = 0.f;
         if (head < G) {
           const Piece q(p.q + (size_t)it.b * p.q_stride + ((size_t)it.h * G + head) * HD, d);
-          q.rotate(turns, [&](int i, float x, float y) {
-            split2(x, y, w[i], rest[i]);
-            sum += x + y;
-          });
+          q.rotate(turns, [&](int i, float x, float y) { split2(x, y, w[i], rest[i]); });
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) w[e] = rest[e] = 0;
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if ((lane & 3) == 0) reinterpret_cast<float*>(slot + 2 * NT * 2048 + 512)[head] = KEY_BIAS * sum;
         uint4* to = reinterpret_cast<uint4*>(slot) + nt * 128 + lane;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -992,8 +968,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
           seek(at + i - i0 + skew);
           if (landed()) {
             const float2 sc = scale[stage];
-            page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, slot + NT * 2048,
-                                reinterpret_cast<const float*>(slot + 2 * NT * 2048 + 512), a, g, t);
+            page_tile<CODE, NT>(ring + stage * STAGE, sc.x, sc.y, qk, qf, slot + NT * 2048, a, g, t);
           }
           release(stage);
         }
