@@ -443,9 +443,10 @@ typedef struct pvlc_kv8_cache {
 /* Scratch of the kv8 calls on caches of up to `pages` pages and `slots` slots,
  * for batches of up to `batch` sequences and `query_heads` heads (0 when they
  * are out of range).  Zeroed once with pvlc_attn_kv8_workspace_init; reusable
- * on one stream, not by calls that may overlap.  After bit 3 it has to be
- * initialised again.  pvlc_attn_kv8_errors waits
- * for the stream, reads and clears the fault word: bit 0 a slot's row count or
+ * on one stream, not by calls that may overlap.  pvlc_attn_kv8_errors waits
+ * for the stream, reads and clears the fault word, and after bit 3, which leaves
+ * tickets behind, the whole of what pvlc_attn_kv8_workspace_init clears; until
+ * then the outputs of later decodes are undefined.  Bit 0 a slot's row count or
  * capacity, bit 1 a rope row, bit 3 a pipeline wait that timed out, bit 4 a
  * page id, bit 5 a slot or parent, bit 6 no free page or slot, bit 7 the
  * input's row range. */

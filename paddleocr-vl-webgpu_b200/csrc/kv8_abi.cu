@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../../include/pvlc_cuda_attn.h"
+#include "pvlc_common.cuh"
 #include "pvlc_internal.h"
 
 namespace pvlc {
@@ -103,8 +104,12 @@ int pvlc_attn_kv8_errors(void* workspace, uint32_t* flags_out, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t flags = 0;
   if (cudaMemcpyAsync(&flags, workspace, 4, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess || cudaMemsetAsync(workspace, 0, 4, s) != cudaSuccess)
+      cudaStreamSynchronize(s) != cudaSuccess)
     return PVLC_CUDA_ERROR;
+  // Blocks that gave up have left tickets behind, by which a later call would join a split unit
+  // before all of its records are written.
+  const size_t clear = flags & kFlagTimeout ? kHeader + kTickets : 4;
+  if (cudaMemsetAsync(workspace, 0, clear, s) != cudaSuccess) return PVLC_CUDA_ERROR;
   *flags_out = flags;
   return flags ? PVLC_DEVICE_FAULT_FLAG : PVLC_OK;
 }

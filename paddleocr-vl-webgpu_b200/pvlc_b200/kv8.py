@@ -155,7 +155,8 @@ class Workspace:
                 self._p, self.nbytes, _raw_stream(self.index)), "pvlc_attn_kv8_workspace_init")
 
     def errors(self) -> int:
-        """Read and clear the fault word (FLAG_* bits); waits for the current stream."""
+        """Read and clear the fault word (FLAG_* bits); waits for the current stream.  After
+        FLAG_TIMEOUT what decode() returned since is undefined, and the workspace is as new."""
         flags = ctypes.c_uint32(0)
         st = abi.lib().pvlc_attn_kv8_errors(self._p, ctypes.byref(flags),
                                             _raw_stream(self.index))
