@@ -345,4 +345,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+// built_for: "<torch version> <Python's cache tag>" of the headers above, which say where a tensor's
+// sizes, strides and address are.  Nothing here may be called under any other.
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpvlc_cuda_attn.so")
@@ -140,10 +141,13 @@ calls = None
 
 def _bind_calls(handle):
     try:
-        import torch  # noqa: F401  (its libraries are what the module links against)
+        import torch               # its libraries are what the module links against
 
         from . import _calls
     except ImportError:
+        return None
+    # the module reads tensors by the layout of the headers that it was compiled with
+    if getattr(_calls, "built_for", None) != f"{torch.__version__} {sys.implementation.cache_tag}":
         return None
     _calls.bind(*[ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in
                   ("pvlc_attn_kv8_store", "pvlc_attn_kv8_decode", "pvlc_attn_kv8_grow",
