@@ -231,6 +231,23 @@ def hypotheses(tok, beam, end_score, end_step, end_beam, done, scores, penalty):
     return [(s, p, why) for s, p, _, why in found[:len(scores)]]
 
 
+def run_chunks(left, chunk, status, queue):
+    """Queue up to `left` steps, a chunk at a time, until all requests are done.  status: (done
+    flags on the host, the event after which they are there) as the prompts left them;
+    queue(steps) queues steps and returns the status behind them.  One chunk is queued ahead of
+    the status that is being looked at."""
+    ahead = None
+    while True:
+        if left > 0:
+            ahead = queue(min(chunk, left))
+            left -= chunk
+        done, event = status
+        event.synchronize()
+        if ahead is None or bool(done.all()):
+            return
+        status, ahead = ahead, None
+
+
 def _decoder(eng, requests, beams, rows, pages, cache_dtype, length_penalty) -> BeamDecoder:
     """The engine's decoder of the last batch shape when it matches, else a new one."""
     key = (requests, beams, rows, pages, cache_dtype, float(length_penalty))
@@ -277,23 +294,12 @@ def generate(eng, images_patches, grids, max_new_tokens, beams, length_penalty, 
         ev[2].record()
     parts = [(_download(dec.step_tok.unsqueeze(0)), _download(dec.step_beam.unsqueeze(0)), None)]
     first_scores = dec.scores.clone() if record else None
-    left = max_new_tokens - 1
-    status = [_download(dec.done)]
-    inflight = 0
-    while True:
-        # one chunk is queued ahead of the one whose end is being looked at
-        while left > 0 and inflight < 2:
-            n = min(chunk, left)
-            tok, beam, rec = dec.run(n, record)
-            parts.append((_download(tok), _download(beam), rec))
-            status.append(_download(dec.done))
-            left -= n
-            inflight += 1
-        host, event = status.pop(0)
-        event.synchronize()
-        if bool(host.all()) or not status:
-            break
-        inflight -= 1
+
+    def queue(steps):
+        tok, beam, rec = dec.run(steps, record)
+        parts.append((_download(tok), _download(beam), rec))
+        return _download(dec.done)
+    run_chunks(max_new_tokens - 1, chunk, _download(dec.done), queue)
     ends = [_download(t) for t in (dec.end_score, dec.end_step, dec.end_beam, dec.done, dec.scores)]
     if ev:
         ev[3].record()
