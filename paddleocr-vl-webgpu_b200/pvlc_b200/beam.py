@@ -249,13 +249,19 @@ def run_chunks(left, chunk, status, queue):
 
 
 def _decoder(eng, requests, beams, rows, pages, cache_dtype, length_penalty) -> BeamDecoder:
-    """The engine's decoder of the last batch shape when it matches, else a new one."""
-    key = (requests, beams, rows, pages, cache_dtype, float(length_penalty))
-    if eng._beam is None or eng._beam[0] != key:
-        eng._beam = None
-        torch.cuda.empty_cache()
-        eng._beam = (key, BeamDecoder(eng, requests, beams, rows, pages, cache_dtype,
-                                      length_penalty))
+    """The engine's decoder of the last batch when it is for as many requests and beams and has
+    room for these rows and pages (what it computes does not depend on how much it has), else
+    a new one, with room for that batch too where only room is missing."""
+    key = (requests, beams, cache_dtype, float(length_penalty))
+    if eng._beam is not None and eng._beam[0] == key:
+        dec = eng._beam[1]
+        if rows <= dec.rows and pages <= dec.cache.pages:
+            return dec
+        rows, pages = max(rows, dec.rows), max(pages, dec.cache.pages)
+        del dec
+    eng._beam = None
+    torch.cuda.empty_cache()
+    eng._beam = (key, BeamDecoder(eng, requests, beams, rows, pages, cache_dtype, length_penalty))
     return eng._beam[1]
 
 
