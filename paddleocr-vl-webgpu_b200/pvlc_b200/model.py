@@ -397,6 +397,8 @@ class OcrEngine:
         uploaded and cut just before that batch is encoded.  Returns generate()'s dict, or
         with beams > 1 (and generate_beam's other options) generate_beam()'s."""
         from . import preprocess
+        if not 1 <= beams <= 32:
+            raise ValueError("beams must be 1 to 32")
         cfgp = preprocess_config or preprocess.MODEL_CONFIG
         ps = cfgp.patch_size
         hosts, sizes = [], []
