@@ -158,8 +158,10 @@ class Workspace:
         """Read and clear the fault word (FLAG_* bits); waits for the current stream.  After
         FLAG_TIMEOUT what decode() returned since is undefined, and the workspace is as new."""
         flags = ctypes.c_uint32(0)
-        st = abi.lib().pvlc_attn_kv8_errors(self._p, ctypes.byref(flags),
-                                            _raw_stream(self.index))
+        # a default stream's handle is the same on every device: it means the current one's
+        with torch.cuda.device(self.device):
+            st = abi.lib().pvlc_attn_kv8_errors(self._p, ctypes.byref(flags),
+                                                _raw_stream(self.index))
         if st not in (abi.OK, abi.DEVICE_FAULT_FLAG):
             abi.check(st, "pvlc_attn_kv8_errors")
         return int(flags.value)
