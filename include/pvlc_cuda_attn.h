@@ -488,6 +488,8 @@ int pvlc_attn_kv8_decode(const pvlc_kv8_cache* cache, uint32_t layer, const pvlc
 /* tokens[slot[b]] += advance[b], then gives every sequence the pages that it
  * lacks for its next ahead[b] rows (full blocks only), lowest free id first,
  * in sequence order.  advance / ahead NULL: advance_by / ahead_by for all.
+ * slot, advance and ahead are read before anything is written (they may be
+ * the cache's tokens).
  * When a slot is bad or named twice, or rows exceed 32 max_pages + 31, the call
  * is flagged and changes nothing; when pages run out, the last sequences'
  * table entries stay -1. */

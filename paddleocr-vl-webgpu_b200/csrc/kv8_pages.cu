@@ -93,9 +93,14 @@ struct GrowParams {
 };
 
 __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowParams g) {
-  extern __shared__ uint32_t sm[];         // the slots, then a bitmap over all slots
+  // The slots, their rows when advanced, the blocks that end within the rows ahead, then a bitmap
+  // over all slots.  The call's arrays are read once, before anything is written: they may be
+  // the cache's own (advance by tokens doubles every sequence).
+  extern __shared__ uint32_t sm[];
   const PageParams& p = g.b;
   int32_t* slot = reinterpret_cast<int32_t*>(sm);
+  int32_t* rows = slot + p.batch;
+  int32_t* ends = rows + p.batch;
   pdl_wait();
   pdl_launch_dependents();
   // the slots and the first pages' counts at once, although few calls need the latter
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
     return bits;
   };
   const uint32_t free_first = free_pages(4 * threadIdx.x);
-  int bad = slots_valid(p, sm + p.batch, slot, first) ? 0 : (int)kFlagSlot;
+  int bad = slots_valid(p, sm + 3 * p.batch, slot, first) ? 0 : (int)kFlagSlot;
   // sequences [b0, b1) are this thread's: ranks follow the sequence order
   const uint32_t per = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS;
   const uint32_t b0 = min(p.batch, threadIdx.x * per), b1 = min(p.batch, b0 + per);
@@ -121,6 +126,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
       const int64_t n = p.tokens[s];
       if (adv < 0 || ahead < 0 || n < 0 || !rows_fit(n + adv + ahead, p.max_pages))
         bad |= kFlagCacheRow;
+      rows[b] = (int32_t)(n + adv);
+      ends[b] = (int32_t)((n + adv + ahead) / PAGE);
     }
   }
   bad = __syncthreads_or(bad) ? (bad ? bad : -1) : 0;
@@ -132,11 +139,9 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
   for (uint32_t b = b0; b < b1; ++b) {
     const int32_t s = slot[b];
     if (s < 0) continue;
-    const int32_t n = p.tokens[s] + (g.advance ? g.advance[b] : g.advance_by);
-    p.tokens[s] = n;
-    const int32_t end = (n + (g.ahead ? g.ahead[b] : g.ahead_by)) / PAGE;
+    p.tokens[s] = rows[b];
     const int32_t* row = p.table + (size_t)s * p.max_pages;
-    for (int32_t j = n / PAGE; j < end; ++j) need += row[j] < 0;
+    for (int32_t j = rows[b] / PAGE; j < ends[b]; ++j) need += row[j] < 0;
   }
   uint32_t total;
   uint32_t rank = block_scan(need, &total);
@@ -160,10 +165,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 1) kv8_grow_kernel(const GrowPar
   for (uint32_t b = b0; b < b1; ++b) {
     const int32_t s = slot[b];
     if (s < 0) continue;
-    const int32_t n = p.tokens[s];
-    const int32_t end = (n + (g.ahead ? g.ahead[b] : g.ahead_by)) / PAGE;
     int32_t* row = p.table + (size_t)s * p.max_pages;
-    for (int32_t j = n / PAGE; j < end; ++j) {
+    for (int32_t j = rows[b] / PAGE; j < ends[b]; ++j) {
       if (row[j] >= 0) continue;
       if (rank < found) {
         const int32_t page = g.list[rank];
@@ -563,7 +566,7 @@ int kv8_grow_launch(const pvlc_kv8_cache& c, const int32_t* slot, uint32_t batch
   g.ahead_by = ahead_by;
   g.list = kv8_scratch(ws);
   return launch(kv8::kv8_grow_kernel, g, dim3(1), kv8::PLAN_THREADS,
-                batch * 4 + (c.slots + 31) / 32 * 4, stream);
+                3 * batch * 4 + (c.slots + 31) / 32 * 4, stream);
 }
 
 int kv8_fork_launch(const pvlc_kv8_cache& c, const int32_t* slot, const int32_t* parent,
