@@ -475,7 +475,8 @@ int pvlc_attn_kv8_store(const pvlc_kv8_cache* cache, uint32_t layer, const pvlc_
  * The rotated key and the value become row tokens % 32 of the tail, attention
  * runs over the tokens / 32 pages and the tail up to that row, and a tail that
  * this row fills is quantised into its page.  query_heads = kv_heads x group,
- * group <= 16.  slot NULL: sequence b is slot b.  tokens is not advanced.  A
+ * group <= 16.  slot NULL: sequence b is slot b.  tokens is not advanced.  out
+ * may not overlap the cache, the workspace or an input.  A
  * sequence with a bad slot, row count or rope row is flagged and its output
  * zero; a bad page id is flagged and its rows read as NaN. */
 int pvlc_attn_kv8_decode(const pvlc_kv8_cache* cache, uint32_t layer, const pvlc_half* q,

@@ -53,6 +53,32 @@ Ranges ranges(const pvlc_kv8_cache& c) {
            (uint64_t)c.slots * c.max_pages * 4, (uint64_t)c.slots * 4, (uint64_t)c.pages * 4}};
 }
 
+// Memory that a call writes: whether other arrays share bytes with it.
+struct Written {
+  uintptr_t at;
+  uint64_t bytes;
+  Written(const void* p, uint64_t n) : at(reinterpret_cast<uintptr_t>(p)), bytes(n) {}
+  bool meets(const void* p, uint64_t n) const {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p);
+    return p && at < x + n && x < at + bytes;
+  }
+  // rows of `n` bytes, `stride` apart
+  bool meets_rows(const void* p, uint64_t rows, uint64_t stride, uint64_t n) const {
+    if (!rows || !meets(p, (rows - 1) * stride + n)) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p);
+    // the last row that begins at or before it, and the one behind that
+    const uint64_t i = at <= x ? 0 : (at - x) / stride;
+    const char* row = static_cast<const char*>(p) + (i < rows ? i : rows - 1) * stride;
+    return meets(row, n) || (i + 1 < rows && meets(row + stride, n));
+  }
+  bool meets(const pvlc_kv8_cache& c) const {
+    const Ranges r = ranges(c);
+    for (int i = 0; i < 6; ++i)
+      if (at < r.at[i] + r.bytes[i] && r.at[i] < at + bytes) return true;
+    return false;
+  }
+};
+
 size_t page_scratch(uint32_t batch, uint32_t slots, uint32_t pages) {
   const size_t fork = 4 + 6 * (size_t)batch + slots, compact = 4 + 2 * (size_t)pages;
   return 4 * (fork > compact ? fork : compact);
@@ -158,6 +184,15 @@ int pvlc_attn_kv8_decode(const pvlc_kv8_cache* cache, uint32_t layer, const pvlc
   if ((st = check_workspace(workspace, workspace_bytes,
                             kv8_decode_scratch_bytes(batch, query_heads, cache->kv_heads))))
     return st;
+  // the output of one sequence is written while another's inputs are read
+  const Written o(out, (uint64_t)batch * query_heads * 256);
+  const uint64_t kv_row = cache->kv_heads * 256ull, table = 3ull * rope_rows * 128 * 4;
+  if (o.meets(*cache) || o.meets_rows(q, batch, q_row_stride * 2ull, query_heads * 256ull) ||
+      o.meets_rows(k_new, batch, kv_row_stride * 2ull, kv_row) ||
+      o.meets_rows(v_new, batch, kv_row_stride * 2ull, kv_row) || o.meets(rope_cos, table) ||
+      o.meets(rope_sin, table) || o.meets(rope_row, batch * 4ull) || o.meets(slot, batch * 4ull) ||
+      o.meets(workspace, workspace_bytes))
+    return PVLC_LENGTH_MISMATCH;
   const Kv8DecodeArgs a{q,         k_new,    v_new, rope_cos, rope_sin,  rope_row, slot,
                         out,       q_row_stride, kv_row_stride, rope_rows, batch, query_heads,
                         workspace};
