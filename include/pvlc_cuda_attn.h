@@ -505,7 +505,7 @@ int pvlc_attn_kv8_grow(const pvlc_kv8_cache* cache, const int32_t* slot, uint32_
  * sharing the parent's full pages and copying its open block in every layer.
  * A sequence that is no parent gives its slot and pages back.  slot_out[b] is
  * the new slot, -1 for none or when slots ran out (flagged); it may not overlap
- * slot or parent.  A bad or repeated slot or a bad parent is flagged and the
+ * slot, parent, the cache or the workspace.  A bad or repeated slot or a bad parent is flagged and the
  * call changes nothing (slot_out = slot). */
 int pvlc_attn_kv8_fork(const pvlc_kv8_cache* cache, const int32_t* slot, const int32_t* parent,
                        uint32_t batch, uint32_t advance_by, int32_t* slot_out, void* workspace,
@@ -514,7 +514,8 @@ int pvlc_attn_kv8_fork(const pvlc_kv8_cache* cache, const int32_t* slot, const i
 /* Copies a cache's live pages (refs > 0), in order, to pages 0, 1, .. of
  * another cache with the same layers, heads and type and at least as many
  * slots; its tables, counts, references and tails are made to match.  *live_out
- * (device, may be NULL) is the number of live pages.  If they, or a slot's
+ * (device, may be NULL, in neither cache nor the workspace) is the number of
+ * live pages.  If they, or a slot's
  * rows, do not fit, the call is flagged, changes nothing and *live_out is -1. */
 int pvlc_attn_kv8_compact(const pvlc_kv8_cache* from, const pvlc_kv8_cache* into,
                           int32_t* live_out, void* workspace, size_t workspace_bytes,

@@ -236,6 +236,8 @@ int pvlc_attn_kv8_fork(const pvlc_kv8_cache* cache, const int32_t* slot, const i
     return PVLC_LENGTH_MISMATCH;           // slot_out is written while slot and parent are read
   if ((st = check_workspace(workspace, workspace_bytes, page_scratch(batch, cache->slots, cache->pages))))
     return st;
+  const Written o(slot_out, span);
+  if (o.meets(*cache) || o.meets(workspace, workspace_bytes)) return PVLC_LENGTH_MISMATCH;
   return kv8_fork_launch(*cache, slot, parent, batch, (int32_t)advance_by, slot_out, workspace,
                          static_cast<cudaStream_t>(stream));
 }
@@ -259,6 +261,9 @@ int pvlc_attn_kv8_compact(const pvlc_kv8_cache* from, const pvlc_kv8_cache* into
     for (int j = 0; j < 6; ++j)
       if (a.at[i] < b.at[j] + b.bytes[j] && b.at[j] < a.at[i] + a.bytes[i])
         return PVLC_LENGTH_MISMATCH;       // nor parts of them
+  const Written o(live_out, 4);
+  if (live_out && (o.meets(*from) || o.meets(*into) || o.meets(workspace, workspace_bytes)))
+    return PVLC_LENGTH_MISMATCH;
   return kv8_compact_launch(*from, *into, live_out, workspace, static_cast<cudaStream_t>(stream));
 }
 

@@ -48,3 +48,18 @@ def test_decode_into_its_rows(i, stride, row):
             assert decode(at) == abi.LENGTH_MISMATCH
             assert decode(at, batch=1) == abi.LENGTH_MISMATCH if b == 0 else True
     assert decode(base - 4 * 4096 + 16) == abi.LENGTH_MISMATCH
+
+
+@pytest.mark.parametrize("name", NAMES + ("ws",))
+def test_fork_and_compact_into_the_cache(name):
+    """slot_out and live_out are written before the tables are read."""
+    other = abi.Kv8CacheStruct(**{n: STEP * (i + 20) for i, n in enumerate(NAMES)}, **SIZES)
+    ws = STEP * 30
+    base, size = (ws, WORKSPACE) if name == "ws" else (getattr(CACHE, name), BYTES[name])
+    for at in (base, base + size - 4, base - 12):
+        assert abi.lib().pvlc_attn_kv8_fork(ctypes.byref(CACHE), STEP * 31, STEP * 32, 4, 1, at, ws,
+                                            WORKSPACE, None) == abi.LENGTH_MISMATCH
+    for a, b in ((CACHE, other), (other, CACHE)):
+        for at in (base, base + size - 4):
+            assert abi.lib().pvlc_attn_kv8_compact(ctypes.byref(a), ctypes.byref(b), at, ws, WORKSPACE,
+                                                   None) == abi.LENGTH_MISMATCH
