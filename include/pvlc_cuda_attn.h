@@ -526,7 +526,8 @@ int pvlc_attn_kv8_compact(const pvlc_kv8_cache* from, const pvlc_kv8_cache* into
  * logits row r * beams + w (f32, or fp16 with half_logits = 1; rows row_stride
  * elements apart).  Scores are computed and compared in f64; equal ones go to
  * the lower beam, then the larger logit, then the lower token.  A NaN logit or
- * candidate counts as -infinity.  The workspace needs no initialisation; one
+ * candidate counts as -infinity.  The outputs overlap neither an input, the
+ * workspace nor one another.  The workspace needs no initialisation; one
  * serves every call of its sizes or smaller ones. */
 #define PVLC_BEAM_MAX_BEAMS 32u
 #define PVLC_BEAM_MAX_TOPK 64u

@@ -297,6 +297,16 @@ int pvlc_lm_head_beam_topk(const void* logits, uint32_t half_logits, uint64_t ro
     return PVLC_MISALIGNED_POINTER;
   if (workspace_bytes < beam_topk_workspace_bytes(batch, beams, vocab, topk))
     return PVLC_WORKSPACE_TOO_SMALL;
+  // a request's results are written while others' scores, logits and lists are read
+  const void* outs[3] = {out_score, out_beam, out_token};
+  const uint64_t n = (uint64_t)batch * topk * 4, unit = half_logits ? 2 : 4;
+  for (int i = 0; i < 3; ++i) {
+    const Written o(outs[i], n);
+    if (o.meets_rows(logits, (uint64_t)batch * beams, row_stride * unit, vocab * unit) ||
+        o.meets(scores, (uint64_t)batch * beams * 4) || o.meets(workspace, workspace_bytes) ||
+        o.meets(outs[(i + 1) % 3], n))
+      return PVLC_LENGTH_MISMATCH;
+  }
   const BeamArgs a{logits, half_logits, row_stride, scores, batch, beams, vocab, topk,
                    workspace, out_score, out_beam, out_token};
   return beam_topk_launch(a, static_cast<cudaStream_t>(stream));

@@ -63,3 +63,21 @@ def test_fork_and_compact_into_the_cache(name):
         for at in (base, base + size - 4):
             assert abi.lib().pvlc_attn_kv8_compact(ctypes.byref(a), ctypes.byref(b), at, ws, WORKSPACE,
                                                    None) == abi.LENGTH_MISMATCH
+
+
+@pytest.mark.parametrize("half", [0, 1])
+def test_beam_outputs(half):
+    """3 requests of 2 beams, 100 logits 128 apart, the best 5."""
+    unit = 2 if half else 4
+    good = [STEP * (40 + i) for i in range(6)]           # logits, scores, workspace, the outputs
+
+    def call(x, s, ws, *outs):
+        return abi.lib().pvlc_lm_head_beam_topk(x, half, 128, s, 3, 2, 100, 5, ws, WORKSPACE, *outs, None)
+    places = [good[0], good[0] + 5 * 128 * unit + 100 * unit - 4, good[0] + 128 * unit + 4, good[0] - 56,
+              good[1], good[1] + 6 * 4 - 4, good[2], good[2] + WORKSPACE - 4]
+    for i in (3, 4, 5):
+        others = [o for o in (3, 4, 5) if o != i]
+        for at in places + [good[o] + d for o in others for d in (0, 56, -56)]:
+            args = list(good)
+            args[i] = at
+            assert call(*args) == abi.LENGTH_MISMATCH, (i, at)
