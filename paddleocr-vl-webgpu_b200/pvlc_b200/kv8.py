@@ -84,7 +84,10 @@ class Cache:
     codes [layers, pages, 2, kv_heads, 32, 128] (torch.float8_e4m3fn or torch.int8), scales
     [layers, pages, kv_heads, 2] f32, tails [layers, slots, 2, kv_heads, 32, 128] fp16, table
     [slots, max_pages], tokens [slots] and refs [pages] int32; all contiguous, on one device.
-    Cache.empty() makes one with no sequences."""
+    Their contents are the caller's to change, the tensors stay: the kernels have their
+    addresses.  Cache.empty() makes one with no sequences."""
+
+    ARRAYS = ("codes", "scales", "tails", "table", "tokens", "refs")
 
     def __init__(self, codes, scales, tails, table, tokens, refs):
         if not isinstance(codes, torch.Tensor) or not codes.is_cuda:
@@ -112,6 +115,11 @@ class Cache:
                                                               tokens, refs)],
                                      L, P, S, M, H, CODE_TYPES[codes.dtype])
         self._p = ctypes.addressof(self._c)
+
+    def __setattr__(self, name, value):
+        if name in self.ARRAYS and getattr(self, name, value) is not value:
+            raise AttributeError(f"a cache keeps its {name} tensor: copy into it instead")
+        super().__setattr__(name, value)
 
     @classmethod
     def empty(cls, layers: int, pages: int, slots: int, max_pages: int, kv_heads: int = 2,
