@@ -133,10 +133,6 @@ _SIGNATURES = {
 EXPORTED = tuple(_SIGNATURES)
 
 _lib = None
-# The compiled argument checks of the 8-bit cache's calls (csrc/py_calls.cpp), once the library
-# is loaded; None where they were not built for this Python and torch: the checks in Python
-# then make the same calls, each about 10 us later.
-calls = None
 
 
 def _bind_calls(handle):
@@ -157,7 +153,7 @@ def _bind_calls(handle):
 
 def lib() -> ctypes.CDLL:
     """Load the in-tree CUDA library (raises if it has not been built)."""
-    global _lib, calls
+    global _lib
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"{LIB_PATH} is missing: build it with __graft_entry__.build() "
@@ -168,8 +164,18 @@ def lib() -> ctypes.CDLL:
             fn.restype = res
             fn.argtypes = args
         _lib = handle
-        calls = _bind_calls(handle)
     return _lib
+
+
+def __getattr__(name):
+    """calls: the compiled argument checks of the 8-bit cache's calls (csrc/py_calls.cpp), bound
+    when they are first asked for, since they need torch and the library does not; None where
+    they were not built for this Python and torch: the checks in Python then make the same
+    calls, each about 10 us later."""
+    if name != "calls":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()["calls"] = found = _bind_calls(lib())
+    return found
 
 
 def status_string(status: int) -> str:

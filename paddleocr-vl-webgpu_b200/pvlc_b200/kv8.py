@@ -193,7 +193,7 @@ def _call(cache, workspace):
 
 
 def _plain(cache, workspace):
-    return abi.calls is not None and type(cache) is Cache and type(workspace) is Workspace
+    return type(cache) is Cache and type(workspace) is Workspace and abi.calls is not None
 
 
 def store(cache: Cache, layer: int, k, v, begin, count, slot, max_count: int,

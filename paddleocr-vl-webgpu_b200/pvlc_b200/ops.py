@@ -436,7 +436,7 @@ def beam_topk(logits, scores, topk: int, workspace: BeamWorkspace | None = None,
     [B, topk] f32, beam [B, topk] int32, token [B, topk] int32), best first, of the candidates
     scores[r, w] + log_softmax(logits[r W + w]).  Equal scores go to the lower beam, then the
     larger logit, then the lower token; NaN counts as -infinity.  out: the three tensors."""
-    if abi.calls is not None and out is None and type(workspace) is BeamWorkspace:
+    if out is None and type(workspace) is BeamWorkspace and abi.calls is not None:
         r = abi.calls.beam_topk(logits, scores, topk, workspace.buffer)
         if type(r) is int:
             abi.check(r, "pvlc_lm_head_beam_topk")

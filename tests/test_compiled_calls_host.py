@@ -44,3 +44,13 @@ def test_the_library_is_built_without_python_or_torch():
     assert got.returncode == 0 and "py_calls" not in got.stdout, got.stdout + got.stderr
     got = make("calls", "PYTHON=/nonexistent")
     assert got.returncode == 0 and "is not built" in got.stdout, got.stdout + got.stderr
+
+
+def test_the_library_loads_without_torch():
+    """A program that uses the C ABI through abi.lib() alone does not wait for torch to load."""
+    code = f"import sys; sys.path.insert(0, {PACKAGE!r}); from pvlc_b200 import abi; abi.lib(); " \
+           "assert 'torch' not in sys.modules; assert abi.calls is not None"
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert got.returncode == 0, got.stderr
+    with pytest.raises(AttributeError):
+        abi.no_such_name
