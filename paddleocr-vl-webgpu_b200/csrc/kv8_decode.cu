@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1)
         Split& u = splits[it.u0 >= y0 ? 1 : 0];
         u.unit = it.b * H + it.h;
         u.blocks = c1 - c0 + 1;
-        u.record = c0 * 2 + (it.u0 >= cuts.begin(c0) ? 1 : 0);
+        u.record = c0 * 2 + 1;
       }
       mbar_arrive(row_full + s);
       if (it.has_tail() && it.sq.rows % PAGE == PAGE - 1) {
