@@ -411,7 +411,8 @@ int pvlc_linear(const pvlc_half* x, uint32_t rows, uint32_t ldx, const pvlc_half
  *
  * Ordering: each of these calls waits for the kernels ahead of it on `stream`
  * before it reads or writes anything, and lets the kernel behind it start
- * early, as all of them allow.  So what they write (tokens, slots, tokens of a
+ * early, as all of them allow (but for store, an ordinary launch, behind which
+ * everything waits for its end).  So what they write (tokens, slots, tokens of a
  * selection) may be read by any call behind them but, directly behind, by one that
  * reads before it waits: pvlc_attn_decode's cache_tokens and rope_row, pvlc_linear's
  * weights.
@@ -524,7 +525,9 @@ int pvlc_attn_kv8_compact(const pvlc_kv8_cache* from, const pvlc_kv8_cache* into
 /* The best topk continuations of every request: out_*[batch, topk], best first,
  * of the beams x vocab candidates scores[r][w] + x[v] - log sum exp(x), x the
  * logits row r * beams + w (f32, or fp16 with half_logits = 1; rows row_stride
- * elements apart).  Scores are computed and compared in f64; equal ones go to
+ * elements apart).  A row's log-sum is of f32 exponentials, summed in f32 by
+ * chunks and in f64 over them, within about 1e-6; scores are f64 sums with it,
+ * compared as such and rounded to f32.  Equal ones go to
  * the lower beam, then the larger logit, then the lower token.  A NaN logit or
  * candidate counts as -infinity.  The outputs overlap neither an input, the
  * workspace nor one another.  The workspace needs no initialisation; one

@@ -11,8 +11,11 @@
 // One pass over the logits, bound by HBM: a block holds a chunk of a row in
 // registers, sums its exponentials against its own maximum and keeps its K best
 // logits as 64-bit keys (ordered logit, then ~token), best first.  A block per
-// request then joins the chunks: the rows' log-sums in f64, so that candidates
-// of two beams that differ by more than 1e-7 are told apart, and the K best.
+// request then joins the chunks: the rows' log-sums, added in f64 over the
+// chunks, and the K best by their f64 scores.  A chunk's own sum is f32 (differences,
+// exponentials within 2^-22, their sum), so a log-sum is within about 1e-6 and
+// candidates of two beams that are further apart than two such errors are told apart;
+// those of one beam share its log-sum and are in the order of their logits.
 //
 // Selection: of any disjoint groups' maxima the K-th largest is a bound that at
 // least K elements reach, so only what reaches it is looked at -- in a chunk, of

@@ -20,15 +20,15 @@
 // the time).  Measured, a layer of 16 query and 2 KV heads, calls back to back:
 //   64 sequences of 606 .. 8,011 rows   34.2 us   4.3 TB/s, 65 % of a copy
 //   16 sequences, 8 KV heads, 4 k .. 8 k rows   37.9 us   4.8 TB/s, 72 %
-//   64 x 4 beams of 1,248 .. 1,499 rows   44.4 us   190 MB through L2, 55 MB of them distinct
+//   64 x 4 beams of 1,248 .. 1,499 rows   46.0 us   190 MB through L2, 55 MB of them distinct
 //   1 sequence of 1,023 rows   9.5 us   bound by its chain of dependent loads
 // Of the 34.2 us 22.3 are the stream at a copy's rate.  4 pass before the first
 // page lands (launch, the sequences' slots, lengths and page ids, each read after
 // the other), 3 in joining the split units, the rest in the uneven end: without
-// its arithmetic the kernel takes 32.3, without its pages 29.4.  The beams are
-// bound by the warps' arithmetic, a page's 48 matrix and some 600 other
-// instructions, each waiting for the one ahead of it more than for a pipe: 32.9
-// and 42.1 (int8, whose conversions are byte permutations).
+// its arithmetic the kernel takes 32.3, without its pages 28.7.  The beams are
+// bound by the warps' arithmetic, a page's 48 matrix and some 630 other
+// instructions, each waiting for the one ahead of it more than for a pipe: 31.0
+// and 43.6 (int8, whose conversions are a byte permutation and a subtraction).
 // More warps an SM do not help (5, 6 and 8 a block: 49, 48 and 56), nor does
 // loading a page that four beams share once, a warp a beam (65: the same work in
 // more code).

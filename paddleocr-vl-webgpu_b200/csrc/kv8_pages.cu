@@ -11,7 +11,7 @@
 //
 // Deciding is one block's work (a few thousand integers); the copies that
 // follow are spread over the GPU.  Measured, 18 layers of 2 heads, calls back to back:
-//   fork and grow of 2 x 4 beams 8.9 us, of 64 x 4 beams 17.7 us (44 MB of open rows, 6.7 us
+//   fork and grow of 2 x 4 beams 8.8 us, of 64 x 4 beams 17.3 us (44 MB of open rows, 6.7 us
 //     of a copy's rate; the rest is three launches, each a chain of dependent loads and scans,
 //     that wait for one another)
 //   compact of 32 sequences, 951 MB read and written, 166 us (5.7 TB/s, 87 % of a copy); of

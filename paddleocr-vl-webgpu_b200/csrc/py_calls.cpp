@@ -1,8 +1,8 @@
 // py_calls.cpp -- the argument checks of pvlc_b200.kv8 and ops.beam_topk as a CPython module
 // (pvlc_b200/_calls): a call whose arguments are all as they should be goes from here to the
 // C ABI; any other returns None, and the Python function checks again, names what is wrong
-// and raises.  A decode step makes such a call per layer, and a call's checks in Python took
-// longer (about 11 us) than most of the kernels that they lead to.
+// and raises.  A decode step that is not captured makes such a call per layer, and a call's
+// checks in Python took longer (about 11 us) than most of the kernels that they lead to.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 

@@ -68,7 +68,8 @@ class BeamDecoder:
         self.q = self.qkv[:, :QW].view(N, c.query_heads, c.head_dim)
         self.k = self.qkv[:, QW:QW + KW].view(N, c.kv_heads, c.head_dim)
         self.v = self.qkv[:, QW + KW:].view(N, c.kv_heads, c.head_dim)
-        # an idle sequence's rows are never written: they stay zero
+        # decode leaves an idle sequence's rows as they are: zero, or the last ones of a request that
+        # is done.  They go through the layers with the others; nothing reads what becomes of them.
         self.ctx = torch.zeros((N, c.query_heads, c.head_dim), dtype=torch.float16, device=dev)
         self.logits = None
         self.graph = None
