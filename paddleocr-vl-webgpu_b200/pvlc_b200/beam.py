@@ -136,9 +136,10 @@ class BeamDecoder:
         with torch.cuda.stream(s):
             self._step()                 # cuBLAS handles and workspaces
         torch.cuda.current_stream().wait_stream(s)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self._step()
+        self.graph = graph               # a capture that failed is not replayed
 
     # ----------------------------------------------------------------- a batch
     def prompts(self, lengths):

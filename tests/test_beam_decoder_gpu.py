@@ -58,3 +58,20 @@ def test_a_batch_that_does_not_fit_gets_another(weights):
     old = eng._beam[1]
     search(eng, SHORT + SHORT[:1], 7)
     assert eng._beam[1] is not old
+
+
+def test_a_capture_that_failed_is_not_replayed(weights, monkeypatch):
+    """The call raises (out of memory, say); the next one captures the step again."""
+    from pvlc_b200 import beam
+    eng, real, calls = M.OcrEngine(CFG, weights), beam.ops.beam_topk, []
+
+    def second_fails(*args, **kw):
+        calls.append(1)
+        if len(calls) == 2:                  # the warm-up's, then the capture's
+            raise RuntimeError("not this time")
+        return real(*args, **kw)
+    monkeypatch.setattr(beam.ops, "beam_topk", second_fails)
+    with pytest.raises(RuntimeError, match="not this time"):
+        search(eng, SHORT, 9)
+    monkeypatch.undo()
+    assert search(eng, SHORT, 9) == search(M.OcrEngine(CFG, weights), SHORT, 9)
